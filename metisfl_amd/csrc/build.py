@@ -90,7 +90,8 @@ def write_ninja() -> str:
         f"-D__HIP_PLATFORM_AMD__ -I{csrc} -I{ROCM}/include {pyinc}",
         f"engine_ldflags = -L{ROCM}/lib -Wl,-rpath,{ROCM}/lib -lamdhip64",
         f"hip_cflags = --offload-arch={ARCH} -O3 -fPIC -std=c++17 -munsafe-fp-atomics -I{csrc} "
-        f"-Wno-unused-result",
+        # packed fp32 arithmetic stays off: some of its forms have given wrong results now and then
+        f"-Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops",
         f"bind_cflags = -O2 -fPIC -std=c++17 -D__HIP_PLATFORM_AMD__ -DUSE_ROCM "
         f"-DTORCH_EXTENSION_NAME=_ops -DTORCH_API_INCLUDE_EXTENSION_H -D_GLIBCXX_USE_CXX11_ABI={abi} "
         f"-I{csrc} {tincs} -I{ROCM}/include {pyinc} -Wno-deprecated-declarations",
