@@ -1,0 +1,87 @@
+// Element types of the any-type operators: 16-byte packs of fp32 / bf16 / fp16
+// that may start at any element (rows of odd width or stride), as floats.
+#pragma once
+#include "kernels/common.h"
+
+namespace mfl {
+
+struct BF16 {
+  uint16_t u;
+};
+typedef _Float16 F16;
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(BF16 v) { return bf2f(v.u); }
+__device__ __forceinline__ float to_f(F16 v) { return (float)v; }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ BF16 from_f<BF16>(float v) {
+  return BF16{f2bf(v)};
+}
+template <>
+__device__ __forceinline__ F16 from_f<F16>(float v) {
+  return (F16)v;
+}
+
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+};
+
+// N elements from p, aligned to the element alone: gfx950's global loads and
+// stores take 16 bytes at any such address.
+template <typename T, int N>
+struct Pack {
+  T e[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+  Pack<T, N> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& v) {
+  __builtin_memcpy(p, &v, sizeof(v));
+}
+
+// Elements c .. c + N - 1 of a row of H (those at or behind H: `fill`).
+template <typename T, int N>
+__device__ __forceinline__ void load_row(const T* row, int c, int H, float fill, float* f) {
+  if (c + N <= H) {
+    const Pack<T, N> v = load_pack<T, N>(row + c);
+#pragma unroll
+    for (int k = 0; k < N; ++k) f[k] = to_f(v.e[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) f[k] = c + k < H ? to_f(row[c + k]) : fill;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* row, int c, int H, const float* f) {
+  if (c + N <= H) {
+    Pack<T, N> v;
+#pragma unroll
+    for (int k = 0; k < N; ++k) v.e[k] = from_f<T>(f[k]);
+    store_pack<T, N>(row + c, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (c + k < H) row[c + k] = from_f<T>(f[k]);
+  }
+}
+
+// Sum over aligned groups of L lanes of a wave.
+template <int L>
+__device__ __forceinline__ float lane_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+}  // namespace mfl

@@ -12,6 +12,9 @@ metisfl/models/keras/keras_model_ops.py:245-283):
 * ``adam``             bias-corrected Adam (Keras default eps 1e-7)
 * ``adam_weight_decay`` Adam + decoupled weight decay
 
+:class:`MultiTensorAdamW` is the Adam / AdamW step over a user module's own
+tensors (any sizes and types, no flat buffer), with states in 32 or 8 bits.
+
 FedProx note: the reference's Keras FedProx keeps its ``vstar`` slot at zero
 (fed_prox.py:44-60); here the anchor is the community
 model received for the round, which is the algorithm's intended semantics.
@@ -141,6 +144,191 @@ class OptRange:
     def run(self) -> None:
         fused_step(self.spec, self.p, self.g, self.m, self.v, self.anchor, self.mirror, self.lr_scale, self.step,
                    zero_grad=self.zero_grad)
+
+
+STATE_BLOCK = 128  # elements that share a scale of MultiTensorAdamW's 8-bit states
+
+
+class MultiTensorAdamW:
+    """Adam / AdamW over a list of tensors, the whole step in two launches (one
+    more for each further 384 tensors; csrc/kernels/multi_adamw.hip).
+
+    ``params``: contiguous float32 or bfloat16 tensors on one device, updated
+    in place; they keep their storage for the optimizer's life.  ``decay``:
+    which of them take ``spec.weight_decay`` (default: all).  ``mirrors``: a
+    bfloat16 copy of each parameter (or None) that the step refreshes.
+    ``lr_scale``: a float32 device tensor of one element that the step
+    multiplies the learning rate with.
+
+    The states are flat buffers, each tensor's segment padded to a multiple of
+    128 elements: ``m`` and ``v`` float32 (``state_bits=32``), or
+    (``state_bits=8``, a quarter of the memory) float8_e4m3fn codes of m and
+    of sqrt(v), whose values are codes times ``m_scale`` / ``v_scale``, one
+    power of two for each 128 elements.  What lies between two codes is
+    rounded up with the chance of its distance, drawn from a mix of ``seed``,
+    step and place: equal seeds give equal results.  bfloat16 parameters are
+    rounded the same way.  ``step_count`` is an int32 device tensor.
+
+    :meth:`step` can be captured into a hipGraph (with the gradients of the
+    captured backward)."""
+
+    def __init__(self, spec: OptimizerSpec, params, *, state_bits: int = 32, decay=None, mirrors=None,
+                 lr_scale: torch.Tensor | None = None, seed: int = 0):
+        if spec.mode not in (OPT_ADAM, OPT_ADAMW):
+            raise ValueError(f"MultiTensorAdamW needs adam or adam_weight_decay, got {spec.kind}")
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        self.spec, self.params, self.state_bits, self.seed = spec, list(params), state_bits, int(seed) & 0xFFFFFFFF
+        if not self.params:
+            raise ValueError("no parameters")
+        n = len(self.params)
+        decay = [True] * n if decay is None else [bool(d) for d in decay]
+        self.mirrors = [None] * n if mirrors is None else list(mirrors)
+        if len(decay) != n or len(self.mirrors) != n:
+            raise ValueError(f"decay and mirrors must have one entry for each of the {n} parameters")
+        dev = self.params[0].device
+        for p, q in zip(self.params, self.mirrors):
+            if p.dtype not in (torch.float32, torch.bfloat16) or not p.is_contiguous() or p.device != dev:
+                raise ValueError("parameters must be contiguous float32 or bfloat16 tensors on one device")
+            if q is not None and (q.dtype != torch.bfloat16 or not q.is_contiguous() or q.device != dev
+                                  or q.numel() != p.numel()):
+                raise ValueError("a mirror must be a contiguous bfloat16 tensor of its parameter's size and device")
+        wd = spec.weight_decay if spec.mode == OPT_ADAMW else 0.0
+        self.weight_decays = [wd if d else 0.0 for d in decay]
+        self.offsets, total = [], 0
+        for p in self.params:
+            self.offsets.append(total)
+            total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
+        zeros = lambda k, t: torch.zeros(k, dtype=t, device=dev)  # noqa: E731
+        st = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        self.m, self.v = zeros(total, st), zeros(total, st)
+        self.m_scale = self.v_scale = None
+        if state_bits == 8:
+            self.m_scale, self.v_scale = (zeros(total // STATE_BLOCK, torch.float32) for _ in range(2))
+        self.step_count = zeros(1, torch.int32)
+        self.lr_scale = lr_scale
+        self._plan = None
+        if dev.type == "cuda":
+            self._plan = ops().AdamPlan(self._storages(), self.mirrors, self.weight_decays, self.m, self.v,
+                                        self.m_scale, self.v_scale, self.step_count, lr_scale, self.offsets)
+
+    def _storages(self) -> list[torch.Tensor]:
+        return [p.detach() for p in self.params]
+
+    @torch.no_grad()
+    def step(self, grads=None) -> None:
+        """One update.  ``grads``: one contiguous float32 / bfloat16 / float16
+        tensor for each parameter (default: their ``.grad``); a parameter whose
+        gradient is None stays as it is, its states too."""
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        s = self.spec
+        if self._plan is not None:
+            self._plan.step(grads, s.learning_rate, s.beta1, s.beta2, s.epsilon, self.seed)
+        else:
+            self._reference(grads)
+
+    # -- states ------------------------------------------------------------------------
+    def state_dict(self) -> dict:
+        """The states' tensors (not copies); see :meth:`load_state_dict`."""
+        d = {"step": self.step_count, "m": self.m, "v": self.v}
+        if self.state_bits == 8:
+            d |= {"m_scale": self.m_scale, "v_scale": self.v_scale}
+        return d
+
+    @torch.no_grad()
+    def load_state_dict(self, state: dict) -> None:
+        """Copies the states of an optimizer over tensors of the same sizes,
+        in the same number of bits."""
+        own = self.state_dict()
+        if set(state) != set(own):
+            raise ValueError(f"states {sorted(state)}, expected {sorted(own)}")
+        for k, t in own.items():
+            if state[k].dtype != t.dtype or state[k].shape != t.shape:
+                raise ValueError(f"state {k} is {state[k].dtype} {tuple(state[k].shape)}, "
+                                 f"expected {t.dtype} {tuple(t.shape)}")
+        for k, t in own.items():
+            t.copy_(state[k])
+
+    # -- the same step on the CPU ------------------------------------------------------
+    def _reference(self, grads) -> None:
+        if len(grads) != len(self.params):
+            raise ValueError(f"got {len(grads)} gradients for {len(self.params)} parameters")
+        for p, g in zip(self.params, grads):
+            if g is None:
+                continue
+            if g.dtype not in (torch.float32, torch.bfloat16, torch.float16) or not g.is_contiguous() \
+                    or g.numel() != p.numel() or g.device != p.device:
+                raise ValueError("a gradient must be contiguous with its parameter's size and device")
+        s, f = self.spec, torch.float32
+        self.step_count += 1
+        t = int(self.step_count)
+        c1 = torch.tensor(1.0 / (1.0 - s.beta1 ** t), dtype=f)
+        c2 = torch.tensor(1.0 / (1.0 - s.beta2 ** t) ** 0.5, dtype=f)
+        lr = torch.tensor(s.learning_rate, dtype=f)
+        if self.lr_scale is not None:
+            lr = lr * self.lr_scale[0]
+        key = _mix32(torch.tensor([(t ^ self.seed) & 0xFFFFFFFF]))
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if g is None or p.numel() == 0:
+                continue
+            n = p.numel()
+            a = self.offsets[i]
+            b = a + -(-n // STATE_BLOCK) * STATE_BLOCK
+            pad = lambda x: torch.nn.functional.pad(x.reshape(-1).to(f), (0, b - a - n))  # noqa: E731,B023
+            at = torch.arange(a, b)
+            bits = _mix32((((at & 0xFFFFFFFF) ^ key) + (at >> 32) * 0x9E3779B1) & 0xFFFFFFFF)
+            g, w = pad(g), pad(p.detach())
+            if self.state_bits == 8:
+                blocks = slice(a // STATE_BLOCK, b // STATE_BLOCK)
+                m = _decode(self.m[a:b], self.m_scale[blocks])
+                v = _decode(self.v[a:b], self.v_scale[blocks]) ** 2
+            else:
+                m, v = self.m[a:b], self.v[a:b]
+            m = m * s.beta1 + g * (1.0 - s.beta1)
+            v = v * s.beta2 + (g * (1.0 - s.beta2)) * g
+            r = v.double().sqrt().float()  # correctly rounded, as the kernel's (torch's fp32 one on the CPU is not)
+            w = w - ((m * c1) / (r * c2 + s.epsilon) + w * self.weight_decays[i]) * lr
+            if self.state_bits == 8:
+                self.m[a:b], self.m_scale[blocks] = _encode(m, bits & 0xFFFF, False)
+                self.v[a:b], self.v_scale[blocks] = _encode(r, bits >> 16, True)
+            else:
+                self.m[a:b], self.v[a:b] = m, v
+            if p.dtype == torch.bfloat16:
+                up = (w.view(torch.int32) + (_mix32(bits) >> 16).int()) & ~0xFFFF
+                w = torch.where(w.isfinite(), up.view(f), w)
+            w = w[:n]
+            p.copy_(w.view(p.shape))
+            if self.mirrors[i] is not None:
+                self.mirrors[i].copy_(w.view(self.mirrors[i].shape))
+
+
+def _mix32(x: torch.Tensor) -> torch.Tensor:
+    """32 mixed bits of whole numbers below 2^32 (int64 tensors)."""
+    x = (x * 0x9E3779B1) & 0xFFFFFFFF
+    x = x ^ (x >> 15)
+    x = (x * 0x6A09E667) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def _decode(code: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    return (code.float().view(-1, STATE_BLOCK) * scale[:, None]).view(-1)
+
+
+def _encode(x: torch.Tensor, dither: torch.Tensor, least: bool):
+    """e4m3 codes and scales (2^E, the block's largest finite value in [128, 256)
+    codes) of x; ``dither`` of 2^16: the chance to go up.  ``least``: values
+    above 0 stay above it."""
+    size = x.abs()
+    top = torch.where(size.isfinite(), size, torch.zeros_like(size)).view(-1, STATE_BLOCK).amax(1)
+    e = torch.where(top > 0, (torch.frexp(top)[1] - 8).clamp(min=-117), torch.tensor(-117, dtype=torch.int32))
+    power = lambda k: ((k + 127) << 23).to(torch.int32).view(torch.float32)  # noqa: E731
+    y = (size.view(-1, STATE_BLOCK) * power(-e)[:, None]).view(-1)
+    low = torch.where(y < 2.0 ** -6, 2.0 ** -6, 0.0)
+    q = (((y + low).view(torch.int32) + (dither << 4).int()) & ~0xFFFFF).view(torch.float32) - low
+    if least:
+        q = torch.where(y > 0, q.clamp(min=2.0 ** -9), q)
+    q = torch.where(y < 512, q, torch.full_like(q, float("nan")))
+    return torch.copysign(q, x).to(torch.float8_e4m3fn), power(e)
 
 
 NO_OPT_TAIL = (None, None, None, None, None, None, None, None, 0, [0.0] * 9, False)

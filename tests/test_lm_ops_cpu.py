@@ -1,0 +1,353 @@
+"""ops.lm and ops.optim.MultiTensorAdamW on CPU tensors: the plain formulas
+against 64-bit definitions and differences, refusals, and a small language
+model trained with all of them."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from metisfl_amd.ops import lm
+from metisfl_amd.ops.optim import STATE_BLOCK, MultiTensorAdamW, OptimizerSpec
+from tests import lm_oracle as oracle
+
+INF = float("inf")
+
+
+def gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- LayerNorm --------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (2, 5, 33), (129,), (0, 4)])
+def test_layer_norm_values(shape):
+    g = gen(1)
+    x = torch.randn(shape, generator=g) * 2 + 0.5
+    w, b = torch.randn(shape[-1], generator=g), torch.randn(shape[-1], generator=g)
+    y, mean, rstd = lm.layer_norm_fwd(x, w, b, 1e-3)
+    o = oracle.layer_norm(x, w, b, 1e-3)
+    for a, k in ((y, "y"), (mean, "mean"), (rstd, "rstd")):
+        assert a.shape == o[k].shape
+        torch.testing.assert_close(a.double(), o[k], rtol=2e-5, atol=2e-5)
+
+
+@pytest.mark.parametrize("affine", ["none", "gamma", "both"])
+def test_layer_norm_gradients_by_differences(affine):
+    g = gen(2)
+    x = torch.randn(3, 2, 5, generator=g, dtype=torch.float64, requires_grad=True)
+    w = torch.randn(5, generator=g, dtype=torch.float64, requires_grad=True) if affine != "none" else None
+    b = torch.randn(5, generator=g, dtype=torch.float64, requires_grad=True) if affine == "both" else None
+    leaves = [t for t in (x, w, b) if t is not None]
+
+    def f(*a):
+        a = list(a) + [None] * (3 - len(a))
+        return lm.layer_norm(a[0], a[1], a[2], 1e-3)
+    assert torch.autograd.gradcheck(f, leaves)
+
+
+def test_layer_norm_refusals():
+    x = torch.zeros(2, 4)
+    with pytest.raises(ValueError, match="gamma"):
+        lm.layer_norm_fwd(x, torch.ones(3))
+    with pytest.raises(ValueError, match="beta without gamma"):
+        lm.layer_norm_fwd(x, None, torch.ones(4))
+    with pytest.raises(ValueError, match="no elements"):
+        lm.layer_norm_fwd(torch.zeros(2, 0))
+    with pytest.raises(ValueError, match="dy"):
+        lm.layer_norm_bwd(torch.zeros(2, 3), x, torch.zeros(2), torch.ones(2))
+
+
+# ---- token log probabilities ---------------------------------------------------------
+@pytest.mark.parametrize("lead,vocab,columns,k", [((4,), 11, 11, 3), ((2, 3), 33, 40, 32), ((1,), 1, 1, 1), ((0,), 5, 5, 2)])
+def test_token_logprobs_values(lead, vocab, columns, k):
+    g = gen(3)
+    z = torch.randn(*lead, columns, generator=g) * 3
+    z[..., vocab:] = 1e30
+    t = torch.randint(-1, columns, lead, generator=g)
+    r = lm.token_logprobs_fwd(z, t, k, vocab)
+    o = oracle.token_logprobs(z, t, k, vocab)
+    assert torch.equal(r.top_ids, o["top_ids"])
+    for n in ("logp", "entropy", "top_logp"):
+        torch.testing.assert_close(getattr(r, n).double(), o[n], rtol=2e-5, atol=2e-5)
+
+
+def test_token_logprobs_gradients_by_differences():
+    g = gen(4)
+    z = torch.randn(2, 3, 7, generator=g, dtype=torch.float64, requires_grad=True)
+    t = torch.tensor([[0, 6, -1], [3, 7, 2]])
+
+    def f(z):
+        r = lm.token_logprobs(z, t, 2, 6)
+        return r.logp, r.entropy, r.top_logp
+    assert torch.autograd.gradcheck(f, (z,))
+
+
+def test_token_logprobs_masks():
+    z = torch.zeros(5, 4)
+    z[0] = -INF                                   # nothing allowed
+    z[1, 1:] = -INF                               # one token left
+    z[2, :2] = torch.finfo(torch.float32).min     # masked by the lowest value
+    z[3, 2] = float("nan")
+    z[4, 1] = INF
+    t = torch.tensor([0, 0, 3, 0, 0])
+    r = lm.token_logprobs_fwd(z, t, 2)
+    assert r.logp[0] == -INF and r.entropy[0] == 0 and r.top_ids[0].tolist() == [0, 1]
+    assert (r.top_logp[0] == -INF).all()
+    assert r.logp[1] == 0 and r.entropy[1] == 0 and r.top_logp[1].tolist() == [0, -INF]
+    assert abs(float(r.logp[2]) + math.log(2)) < 1e-6 and r.top_ids[2].tolist() == [2, 3]
+    assert r.logp[3].isnan() and r.entropy[3].isnan() and r.top_ids[3].tolist() == [0, 1]
+    assert r.entropy[4].isnan() and int(r.top_ids[4, 0]) == 1
+    one = torch.ones(5)
+    d = lm.token_logprobs_bwd(z, t, r.stats, one, one, torch.ones(5, 2), r.top_ids)
+    assert (d[0] == 0).all() and d[:3].isfinite().all() and d[3].isnan().any()
+
+
+def test_token_logprobs_refusals():
+    z, t = torch.zeros(2, 4), torch.zeros(2, dtype=torch.int64)
+    for bad in (0, 5):
+        with pytest.raises(ValueError, match="vocab"):
+            lm.token_logprobs_fwd(z, t, vocab=bad)
+    for k in (-1, 5, 33):
+        with pytest.raises(ValueError, match="top_k"):
+            lm.token_logprobs_fwd(z, t, k)
+    with pytest.raises(ValueError, match="targets"):
+        lm.token_logprobs_fwd(z, t[:1])
+    with pytest.raises(TypeError, match="int64"):
+        lm.token_logprobs_fwd(z, t.float())
+    r = lm.token_logprobs_fwd(z, t, 2)
+    with pytest.raises(ValueError, match="top_ids"):
+        lm.token_logprobs_bwd(z, t, r.stats, d_top=torch.zeros(2, 2))
+    with pytest.raises(ValueError, match="stats"):
+        lm.token_logprobs_bwd(z, t, r.stats[:1], r.logp)
+    with pytest.raises(ValueError, match="d_logp"):
+        lm.token_logprobs_bwd(z, t, r.stats, torch.zeros(3))
+
+
+# ---- AdamW ------------------------------------------------------------------------------
+SPEC = OptimizerSpec("adam_weight_decay", 1e-2, weight_decay=0.1, epsilon=1e-6)
+
+
+def test_adamw_32_bits_against_definition():
+    g = gen(5)
+    sizes = [1, 5, 127, 128, 300, 0]
+    params = [torch.randn(n, generator=g) for n in sizes]
+    grads = [[torch.randn(n, generator=g) for n in sizes] for _ in range(3)]
+    decay = [True, False, True, True, False, True]
+    want = [(p.double(), torch.zeros(p.numel()).double(), torch.zeros(p.numel()).double()) for p in params]
+    opt = MultiTensorAdamW(SPEC, params, decay=decay)
+    for t, gs in enumerate(grads, 1):
+        opt.step(gs)
+        want = [oracle.adamw(p, x, m, v, t, 1e-2, 0.9, 0.999, 1e-6, 0.1 if d else 0.0)
+                for (p, m, v), x, d in zip(want, gs, decay)]
+    for p, (w, _, _) in zip(params, want):
+        # three steps of a few roundings of values up to 4
+        torch.testing.assert_close(p.double(), w, rtol=1e-6, atol=2e-6)
+    assert int(opt.step_count) == 3
+
+
+def test_adamw_skips_missing_gradients_and_refreshes_mirrors():
+    params = [torch.ones(3), torch.ones(130)]
+    mirrors = [None, torch.zeros(130, dtype=torch.bfloat16)]
+    opt = MultiTensorAdamW(SPEC, params, mirrors=mirrors, state_bits=8)
+    opt.step([None, torch.full((130,), 0.5)])
+    assert (params[0] == 1).all() and (params[1] != 1).all()
+    assert torch.equal(mirrors[1], params[1].to(torch.bfloat16))
+    assert (opt.m[:STATE_BLOCK].float() == 0).all()
+
+
+@pytest.mark.parametrize("scale", [1e-38, 1e-12, 1.0, 1e12, 1e30])
+def test_state_codes_keep_the_mean(scale):
+    """A value between two codes is rounded up with the chance of its
+    distance: the mean over N draws is off by the deviation of a mean, at most
+    a code (an eighth of the value, or 2^-9 of the scale) / (2 sqrt N)."""
+    from metisfl_amd.ops.optim import _decode, _encode
+    n, reps = STATE_BLOCK, 4096
+    x = scale * torch.logspace(0, -6, n)
+    g = gen(6)
+    total = torch.zeros(n, dtype=torch.float64)
+    for _ in range(reps):
+        code, s = _encode(x, torch.randint(0, 1 << 16, (n,), generator=g), False)
+        total += _decode(code, s).double()
+    step = torch.maximum(x.double() / 8, s.double() * 2.0 ** -9)
+    # six deviations of the mean, and the dither's own step of 2^-16
+    bound = step * (6 / (2 * reps ** 0.5) + 2.0 ** -15)
+    assert ((total / reps - x.double()).abs() <= bound).all()
+
+
+def test_state_codes_of_special_values():
+    from metisfl_amd.ops.optim import _decode, _encode
+    x = torch.zeros(3 * STATE_BLOCK)
+    x[0], x[1], x[2] = INF, float("nan"), 3.0       # others of the block keep a scale of finite values
+    x[2 * STATE_BLOCK] = 1.0
+    x[2 * STATE_BLOCK + 1] = 1e-30                  # far below its block's largest
+    code, s = _encode(x, torch.zeros(x.numel(), dtype=torch.int64), True)
+    y = _decode(code, s)
+    assert y[0].isnan() and y[1].isnan() and y[2] == 3.0
+    assert (y[STATE_BLOCK:2 * STATE_BLOCK] == 0).all()
+    assert y[2 * STATE_BLOCK] == 1.0 and 0 < y[2 * STATE_BLOCK + 1] < 1e-4
+
+
+def test_adamw_8_bits_follows_32_bits():
+    """A constant gradient: both move every element by the same sign, and the
+    8-bit second moment follows the true one (a nearest rounding would stay
+    at its first value)."""
+    n = 512
+    g = torch.exp(torch.randn(n, generator=gen(7)))
+    a, b = torch.zeros(n), torch.zeros(n)
+    oa = MultiTensorAdamW(OptimizerSpec("adam", 1e-3), [a])
+    ob = MultiTensorAdamW(OptimizerSpec("adam", 1e-3), [b], state_bits=8)
+    for _ in range(200):
+        oa.step([g])
+        ob.step([g])
+    v = (ob.v.float().view(-1, STATE_BLOCK) * ob.v_scale[:, None]).view(-1) ** 2
+    # mean over 512 elements of a value that wanders by about a code (an
+    # eighth of sqrt v: a quarter of v at most)
+    assert abs(float((v / oa.v).mean()) - 1) < 0.25
+    assert abs(float((b / a).mean()) - 1) < 0.25
+
+
+def test_adamw_states_round_trip():
+    g = gen(8)
+    a, b = [torch.randn(200, generator=g)], [torch.zeros(200)]
+    oa = MultiTensorAdamW(SPEC, a, state_bits=8, seed=3)
+    x = torch.randn(200, generator=g)
+    oa.step([x])
+    b[0].copy_(a[0])
+    ob = MultiTensorAdamW(SPEC, b, state_bits=8, seed=3)
+    ob.load_state_dict(oa.state_dict())
+    oa.step([x])
+    ob.step([x])
+    assert torch.equal(a[0], b[0]) and torch.equal(oa.m.view(torch.uint8), ob.m.view(torch.uint8))
+
+
+def test_adamw_refusals():
+    p = [torch.zeros(4)]
+    with pytest.raises(ValueError, match="adam"):
+        MultiTensorAdamW(OptimizerSpec("vanilla_sgd", 0.1), p)
+    with pytest.raises(ValueError, match="state_bits"):
+        MultiTensorAdamW(SPEC, p, state_bits=16)
+    with pytest.raises(ValueError, match="no parameters"):
+        MultiTensorAdamW(SPEC, [])
+    with pytest.raises(ValueError, match="contiguous"):
+        MultiTensorAdamW(SPEC, [torch.zeros(4, 4).t()[:, :2]])
+    with pytest.raises(ValueError, match="contiguous float32"):
+        MultiTensorAdamW(SPEC, [torch.zeros(4, dtype=torch.float16)])
+    with pytest.raises(ValueError, match="mirror"):
+        MultiTensorAdamW(SPEC, p, mirrors=[torch.zeros(4)])
+    with pytest.raises(ValueError, match="one entry"):
+        MultiTensorAdamW(SPEC, p, decay=[True, False])
+    opt = MultiTensorAdamW(SPEC, p)
+    with pytest.raises(ValueError, match="gradient"):
+        opt.step([torch.zeros(5)])
+    with pytest.raises(ValueError, match="gradients"):
+        opt.step([])
+    with pytest.raises(ValueError, match="states"):
+        opt.load_state_dict({"m": opt.m})
+    with pytest.raises(ValueError, match="state m"):
+        opt.load_state_dict({**opt.state_dict(), "m": torch.zeros(5)})
+
+
+# ---- together ------------------------------------------------------------------------------
+class Norm(torch.nn.Module):
+    def __init__(self, width):
+        super().__init__()
+        self.gamma = torch.nn.Parameter(torch.ones(width))
+        self.beta = torch.nn.Parameter(torch.zeros(width))
+
+    def forward(self, x):
+        return lm.layer_norm(x, self.gamma, self.beta, 1e-5)
+
+
+class TinyLM(torch.nn.Module):
+    """Next-token model with a tied output: embedding, norm, mixing, norm."""
+
+    def __init__(self, vocab=50, width=24):
+        super().__init__()
+        self.emb = torch.nn.Embedding(vocab, width)
+        self.n1, self.mix, self.n2 = Norm(width), torch.nn.Linear(width, width), Norm(width)
+
+    def forward(self, tokens):
+        h = self.n1(self.emb(tokens))
+        h = self.n2(h + torch.tanh(self.mix(h)))
+        return h @ self.emb.weight.t()
+
+
+def loss_of(logits, targets):
+    r = lm.token_logprobs(logits, targets)
+    return -r.logp.sum() / (targets >= 0).sum()
+
+
+def check_step_gradients(device):
+    """One step's gradients against the same model in 64 bits with torch's own operators."""
+    torch.manual_seed(0)
+    net = TinyLM()
+    tokens = torch.randint(0, 50, (4, 9))
+    targets = torch.roll(tokens, -1, 1)
+    targets[:, -1] = -1
+    want = TinyLM().double()
+    want.load_state_dict(net.state_dict())
+    h = torch.nn.functional.layer_norm(want.emb(tokens), (24,), want.n1.gamma, want.n1.beta, 1e-5)
+    h = torch.nn.functional.layer_norm(h + torch.tanh(want.mix(h)), (24,), want.n2.gamma, want.n2.beta, 1e-5)
+    logits = h @ want.emb.weight.t()
+    ref = torch.nn.functional.cross_entropy(logits.flatten(0, 1), targets.flatten(), ignore_index=-1)
+    ref.backward()
+    net = net.to(device)
+    loss = loss_of(net(tokens.to(device)), targets.to(device))
+    loss.backward()
+    assert abs(float(loss) - float(ref)) < 1e-5
+    for (n, p), q in zip(net.named_parameters(), want.parameters()):
+        # fp32 sums of up to 50 x 36 products
+        torch.testing.assert_close(p.grad.cpu().double(), q.grad, rtol=1e-4, atol=1e-5 * float(q.grad.abs().max()), msg=n)
+
+
+def test_model_gradients():
+    check_step_gradients("cpu")
+
+
+def fit_def():
+    from metisfl_amd.models.model_def import TorchModelDef
+
+    class LMDef(TorchModelDef):
+        """A user model that keeps its own loop, with the 8-bit optimizer."""
+
+        def get_model(self):
+            return TinyLM()
+
+        def loss(self, outputs, targets):
+            return loss_of(outputs, targets)
+
+        def fit(self, model, dataset, epochs):
+            dev = next(model.parameters()).device
+            if getattr(self, "opt", None) is None:
+                params = [p for p in model.parameters()]
+                self.opt = MultiTensorAdamW(OptimizerSpec("adam_weight_decay", 1e-2, weight_decay=0.01, epsilon=1e-6),
+                                            params, state_bits=8, decay=[p.dim() > 1 for p in params])
+            x, y = torch.as_tensor(dataset.get_x()).to(dev), torch.as_tensor(dataset.get_y()).to(dev)
+            for _ in range(epochs):
+                for p in self.opt.params:
+                    p.grad = None
+                self.loss(model(x), y).backward()
+                self.opt.step()
+    return LMDef()
+
+
+def check_user_fit(device):
+    from metisfl_amd.models.torch_net import TorchNet
+    rng = np.random.default_rng(0)
+    x = rng.integers(0, 50, (8, 9))
+    y = np.roll(x, -1, 1)
+    y[:, -1] = -1
+    net = TorchNet(fit_def(), 8, device=device)
+    ds = net.make_dataset(x, y)
+    before = net.state.params32.clone()
+    net.train_steps(ds, 3)
+    assert int(net.model_def.opt.step_count) == 3
+    after = net.state.params32
+    assert after.isfinite().all() and not torch.equal(before, after)
+    # every update is at most lr * (a few + decay)
+    assert float((after - before).abs().max()) < 3 * 1e-2 * 11
+    assert math.isfinite(net.evaluate(ds)["loss"])
+
+
+def test_user_fit():
+    check_user_fit("cpu")
