@@ -76,12 +76,40 @@ __device__ __forceinline__ void store_row(T* row, int c, int H, const float* f) 
   }
 }
 
-// Sum over aligned groups of L lanes of a wave.
+// Reductions over a wave's rows of 16 lanes by DPP rotations (every lane gets
+// the result; a rotation costs a VALU instruction where a shuffle goes through
+// LDS), and over all 64 lanes by four lane reads more.  The lanes of a row (of
+// the wave) must all be active.
+template <int N>
+__device__ __forceinline__ float row_ror(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+__device__ __forceinline__ float sum16(float v) {
+  v += row_ror<8>(v);
+  v += row_ror<4>(v);
+  v += row_ror<2>(v);
+  return v + row_ror<1>(v);
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, row_ror<8>(v));
+  v = fmaxf(v, row_ror<4>(v));
+  v = fmaxf(v, row_ror<2>(v));
+  return fmaxf(v, row_ror<1>(v));
+}
+// Sum over aligned groups of L (16 or 64) lanes.
 template <int L>
 __device__ __forceinline__ float lane_sum(float v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  static_assert(L == 16 || L == 64, "a row of 16 lanes or a wave");
+  v = sum16(v);
+  if constexpr (L == 64) v = (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
   return v;
+}
+__device__ __forceinline__ float max64(float v) {
+  v = max16(v);
+  return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
 }
 
 }  // namespace mfl

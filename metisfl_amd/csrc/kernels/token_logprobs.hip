@@ -25,43 +25,64 @@
 namespace mfl {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kList = 1024;  // candidates of a row (LDS)
 
-// Running maximum, sum of exp(x - m) and sum of exp(x - m) (x - m).
+// Running maximum m, sum of exp(x - m) and sum of exp(x - m) (x - m) log2 e.
+// exp(x - m) = exp2(x L - fl(m L)) with L = log2 e is one fused multiply-add
+// and one v_exp_f32; what fl(m L) is rounded by is a factor common to the sum,
+// taken out by soft_exact at the end, so the error of a term is a few times
+// 2^-24 of |x - m|, not of |x|.  Where m L would leave fp32 (rows masked with
+// the lowest value throughout) the difference is taken first.
 struct Soft {
   float m, s, t;
 };
-__device__ __forceinline__ Soft soft_none() { return {-INFINITY, 0.f, 0.f}; }
-// t of a sum whose maximum goes from m to M: each (x - m) grows by (m - M)
+constexpr float kHuge = 1e38f;
+__device__ __forceinline__ float scaled_max(float m) { return m == -INFINITY ? 0.f : m * kLog2e; }
+// the sums from maximum a.m to M >= a.m: each (x - m) log2 e grows by d
 __device__ __forceinline__ void soft_raise(Soft& a, float M) {
-  if (a.s != 0.f) {
-    const float d = a.m - M, c = exp2f(d * kLog2e);
+  if (a.s != 0.f) {  // (s is 0 only where nothing but -inf was added)
+    const float d = (a.m - M) * kLog2e, c = __builtin_amdgcn_exp2f(d);
     a.t = c * (a.t + (c > 0.f ? d * a.s : 0.f));
     a.s *= c;
   }
   a.m = M;
 }
-__device__ __forceinline__ Soft soft_join(Soft a, Soft b) {
-  const float M = fmaxf(a.m, b.m);
-  soft_raise(a, M);
-  soft_raise(b, M);
-  return {M, a.s + b.s, a.t + b.t};
+__device__ __forceinline__ void soft_exact(Soft& a) {
+  const float ml = scaled_max(a.m);
+  const float off = fabsf(a.m) > kHuge ? 0.f : fmaf(a.m, kLog2e, -ml);  // x L - fl(m L) - off = (x - m) L
+  const float c = fmaf(-off, kLn2, 1.f);                              // 2^-off
+  a.t = c * fmaf(-off, a.s, a.t);
+  a.s *= c;
 }
-// N more elements (fill: -inf)
+// N more elements (fill: -inf) with the largest of them
 template <int N>
-__device__ __forceinline__ void soft_add(Soft& a, const float* x) {
-  float M = a.m;
+__device__ __forceinline__ void soft_add(Soft& a, const float* x, float largest) {
+  if (largest > a.m) soft_raise(a, largest);
+  if (fabsf(a.m) > kHuge && a.m != -INFINITY) {
 #pragma unroll
-  for (int k = 0; k < N; ++k) M = fmaxf(M, x[k]);
-  if (M > a.m) soft_raise(a, M);
-  const float m = a.m == -INFINITY ? 0.f : a.m;
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const float d = x[k] - m, e = __builtin_amdgcn_exp2f(d * kLog2e);
-    a.s += e;
-    a.t = fmaf(e, fmaxf(d, -1e4f), a.t);  // a masked logit adds 0, not 0 * -inf
+    for (int k = 0; k < N; ++k) {
+      const float d = (x[k] - a.m) * kLog2e, e = __builtin_amdgcn_exp2f(d);
+      a.s += e;
+      a.t = fmaf(e, fmaxf(d, -1e4f), a.t);
+    }
+    return;
   }
+  const float ml = scaled_max(a.m);
+  float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; k += 2) {
+    const float d0 = fmaf(x[k], kLog2e, -ml), e0 = __builtin_amdgcn_exp2f(d0);
+    s0 += e0;
+    t0 = fmaf(e0, fmaxf(d0, -1e4f), t0);  // a masked logit adds 0, not 0 * -inf
+    if (k + 1 < N) {
+      const float d1 = fmaf(x[k + 1], kLog2e, -ml), e1 = __builtin_amdgcn_exp2f(d1);
+      s1 += e1;
+      t1 = fmaf(e1, fmaxf(d1, -1e4f), t1);
+    }
+  }
+  a.s += s0 + s1;
+  a.t += t0 + t1;
 }
 
 // Order of the alternatives as whole numbers: larger logit first, then lower
@@ -83,8 +104,8 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 template <int THREADS>
 struct RowShared {
   float m[16], s[16], t[16];
-  int group[64];
-  int bound, count;
+  float group[64];
+  int count;
   uint64_t best[16], top[kTopMax], list[THREADS > 64 ? kList : 256];
 };
 
@@ -94,39 +115,98 @@ __device__ __forceinline__ void row_sync() {
   else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"), __builtin_amdgcn_wave_barrier();
 }
 
-// The K largest keys of x[0 .. n) into sh.top, each thread holding the largest
-// order `mine` of its own elements (those its loop visits).
+// What a thread saw of the row: its largest element, the batch (packs b * THREADS
+// + tid, ... of its loop) that had it, and the largest of its other batches.
+struct Seen {
+  float largest, others;
+  int batch;
+};
+constexpr int kUnroll = 4;  // packs of a batch: the loads in flight of a thread
+
+// The packs of batch `b` of a row of `n` elements: element u * N + k of f is
+// x[((b * kUnroll + u) * THREADS + tid) * N + k], -inf behind the last whole pack.
 template <typename T, int THREADS>
-__device__ void row_top(const T* x, int n, uint32_t first, int K, int mine, RowShared<THREADS>& sh) {
+struct Batch {
+  static constexpr int N = Vec<T>::N;
+  Pack<T, N> v[kUnroll];
+  __device__ __forceinline__ void load(const T* x, int b, int packs) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = (b * kUnroll + u) * THREADS + (int)(threadIdx.x % THREADS);
+      v[u] = load_pack<T, N>(x + (int64_t)(i < packs ? i : packs - 1) * N);
+    }
+  }
+  __device__ __forceinline__ void get(int b, int packs, float* f) const {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) f[u * N + k] = to_f(v[u].e[k]);
+    }
+    if ((b + 1) * kUnroll * THREADS > packs) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = (b * kUnroll + u) * THREADS + (int)(threadIdx.x % THREADS);
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[u * N + k] = i < packs ? f[u * N + k] : -INFINITY;
+      }
+    }
+  }
+};
+
+// The K largest keys of x[0 .. n) into sh.top (ids counted from `first`).
+template <typename T, int THREADS>
+__device__ void row_top(const T* x, int n, uint32_t first, int K, Seen seen, RowShared<THREADS>& sh) {
   constexpr int N = Vec<T>::N, GROUP = THREADS / 64, CAP = THREADS > 64 ? kList : 256;
   const int tid = threadIdx.x % THREADS;
-  int g = mine;
-#pragma unroll
-  for (int o = 1; o < GROUP; o <<= 1) g = max(g, __shfl_xor(g, o, 64));
-  if (tid % GROUP == 0) sh.group[tid / GROUP] = g;
-  if (tid == 0) sh.count = 0;
-  row_sync<THREADS>();
-  if (tid < 64) {
-    const int v = sh.group[tid];
-    int rank = 0;
-    for (int j = 0; j < 64; ++j) {
-      const int w = sh.group[j];
-      rank += w > v || (w == v && j < tid);
-    }
-    if (rank == K - 1) sh.bound = v;
+  // 64 groups of neighbouring threads; the K-th largest of their maxima
+  float g = seen.largest;
+  if constexpr (GROUP == 16) {
+    g = max16(g);
+  } else if constexpr (GROUP == 4) {
+    g = fmaxf(g, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(g), 0xb1, 0xf, 0xf, false)));  // 1 0 3 2
+    g = fmaxf(g, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(g), 0x4e, 0xf, 0xf, false)));  // 2 3 0 1
   }
+  if constexpr (GROUP > 1) {
+    if (tid % GROUP == 0) sh.group[tid / GROUP] = g;
+    if (tid == 0) sh.count = 0;
+    row_sync<THREADS>();
+    g = sh.group[tid & 63];
+  } else if (tid == 0) {
+    sh.count = 0;
+  }
+  int above = 0;  // groups above this lane's
+#pragma unroll
+  for (int j = 0; j < 64; ++j) above += lane_of(g, j) > g;
+  const float least = -max64(above < K ? -g : -INFINITY);
+  const int bound = order_of(least);
   row_sync<THREADS>();
-  const int bound = sh.bound;
-  if (mine >= bound) {
-    for (int c = tid * N; c < n; c += THREADS * N)
-      for (int k = 0; k < N; ++k)
-        if (c + k < n) {
-          const int o = order_of(to_f(x[c + k]));
-          if (o >= bound) {
+  // threads that saw an element of that size list theirs
+  const int packs = n / N, batches = (packs + THREADS * kUnroll - 1) / (THREADS * kUnroll);
+  if (packs && order_of(seen.largest) >= bound) {
+    const bool one = seen.batch >= 0 && order_of(seen.others) < bound;
+    for (int b = one ? seen.batch : 0; b < (one ? seen.batch + 1 : batches); ++b) {
+      Batch<T, THREADS> v;
+      v.load(x, b, packs);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = (b * kUnroll + u) * THREADS + tid;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int o = order_of(to_f(v.v[u].e[k]));
+          if (i < packs && o >= bound) {
             const int at = atomicAdd(&sh.count, 1);
-            if (at < CAP) sh.list[at] = rank_key(o, first + c + k);
+            if (at < CAP) sh.list[at] = rank_key(o, first + (uint32_t)(i * N + k));
           }
         }
+      }
+    }
+  }
+  if (packs * N + tid < n) {  // behind the last whole pack: one element of the first threads
+    const int o = order_of(to_f(x[packs * N + tid]));
+    if (o >= bound) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < CAP) sh.list[at] = rank_key(o, first + (uint32_t)(packs * N + tid));
+    }
   }
   row_sync<THREADS>();
   const int count = sh.count;
@@ -134,6 +214,7 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, int mine, RowS
     for (int i = tid; i < count; i += THREADS) {
       const uint64_t v = sh.list[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < count; ++j) rank += sh.list[j] > v;
       if (rank < K) sh.top[rank] = v;
     }
@@ -144,7 +225,7 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, int mine, RowS
   for (int k = 0; k < K; ++k) {
     uint64_t best = 0;
     for (int c = tid; c < n; c += THREADS) {
-      const uint64_t v = rank_key(order_of(to_f(x[c])), first + c);
+      const uint64_t v = rank_key(order_of(to_f(x[c])), first + (uint32_t)c);
       if (v < last && v > best) best = v;
     }
 #pragma unroll
@@ -163,44 +244,56 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, int mine, RowS
   row_sync<THREADS>();
 }
 
-// One pass over x[0 .. n): the row's (or its part's) running sums in all
-// threads of the row, and the largest order of this thread's elements.
+// One pass over x[0 .. n): the row's sums in all its threads, and what this
+// thread saw.
 template <typename T, int THREADS>
-__device__ __forceinline__ Soft row_pass(const T* x, int n, int& mine, RowShared<THREADS>& sh) {
-  constexpr int N = Vec<T>::N, UNROLL = 4;
+__device__ __forceinline__ Soft row_pass(const T* x, int n, Seen& seen, RowShared<THREADS>& sh) {
+  constexpr int N = Vec<T>::N;
   const int tid = threadIdx.x % THREADS;
-  Soft a = soft_none();
-  float largest = -INFINITY;
-  int c = tid * N;
-  for (; c + (UNROLL - 1) * THREADS * N + N <= n; c += UNROLL * THREADS * N) {
-    float f[UNROLL][N];
+  const int packs = n / N, batches = (packs + THREADS * kUnroll - 1) / (THREADS * kUnroll);
+  Soft a = {-INFINITY, 0.f, 0.f};
+  seen = {-INFINITY, -INFINITY, -1};
+  float tail = -INFINITY;
+  if (packs * N + tid < n) tail = to_f(x[packs * N + tid]);
+  Batch<T, THREADS> v;
+  if (batches) v.load(x, 0, packs);
+  for (int b = 0; b < batches; ++b) {
+    float f[kUnroll * N];
+    v.get(b, packs, f);
+    if (b + 1 < batches) v.load(x, b + 1, packs);  // in flight while this batch is added
+    float largest = f[0];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) load_row<T, N>(x, c + u * THREADS * N, n, -INFINITY, f[u]);
-    soft_add<UNROLL * N>(a, &f[0][0]);
+    for (int k = 1; k < kUnroll * N; ++k) largest = fmaxf(largest, f[k]);
+    if (largest > seen.largest) {
+      seen.others = seen.largest;
+      seen.largest = largest;
+      seen.batch = b;
+    } else {
+      seen.others = fmaxf(seen.others, largest);
+    }
+    soft_add<kUnroll * N>(a, f, largest);
   }
-  for (; c < n; c += THREADS * N) {
-    float f[N];
-    load_row<T, N>(x, c, n, -INFINITY, f);
-    soft_add<N>(a, f);
-  }
-  largest = a.m;
-  mine = order_of(largest);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const Soft b = {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)};
-    a = soft_join(a, b);
-  }
+  soft_add<1>(a, &tail, tail);
+  soft_exact(a);
+  const float wave = max64(a.m);
+  soft_raise(a, wave);
+  a.s = lane_sum<64>(a.s);
+  a.t = lane_sum<64>(a.t);
   if constexpr (THREADS > 64) {
-    const int w = threadIdx.x >> 6;
+    const int w = threadIdx.x >> 6, j = threadIdx.x & 15;
     if ((threadIdx.x & 63) == 0) {
       sh.m[w] = a.m;
       sh.s[w] = a.s;
       sh.t[w] = a.t;
     }
     __syncthreads();
-    a = {sh.m[0], sh.s[0], sh.t[0]};
-    for (int i = 1; i < THREADS / 64; ++i) a = soft_join(a, {sh.m[i], sh.s[i], sh.t[i]});
+    a = {-INFINITY, 0.f, 0.f};
+    if (j < THREADS / 64) a = {sh.m[j], sh.s[j], sh.t[j]};
+    soft_raise(a, max16(a.m));
+    a.s = sum16(a.s);
+    a.t = sum16(a.t);
   }
+  a.t *= kLn2;
   return a;
 }
 
@@ -210,16 +303,13 @@ __device__ __forceinline__ int64_t target_of(const int64_t* t64, const int32_t* 
 
 // Results of a row from its sums (and sh.top), by the row's threads.
 template <typename T, int THREADS>
-__device__ __forceinline__ void row_write(const TokenLogprobs& a, const T* x, int64_t row, Soft r,
+__device__ __forceinline__ void row_write(const TokenLogprobs& a, int64_t row, Soft r, bool has, float given,
                                           RowShared<THREADS>& sh) {
   const int tid = threadIdx.x % THREADS;
   const float logs = logf(r.s);
   const bool empty = r.m == -INFINITY && r.s == 0.f;
   if (tid == 0) {
-    const int64_t t = target_of(a.target64, a.target32, row);
-    float lp = 0.f;
-    if (t >= 0 && t < a.V) lp = empty ? -INFINITY : (to_f(x[t]) - r.m) - logs;
-    a.logp[row] = lp;
+    a.logp[row] = !has ? 0.f : empty ? -INFINITY : (given - r.m) - logs;
     const float entropy = empty ? 0.f : logs - r.t / r.s;
     a.entropy[row] = entropy;
     a.stats[3 * row] = r.m;
@@ -240,28 +330,33 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void logprobs_kernel
   RowShared<THREADS>& sh = shared[threadIdx.x / THREADS];
   for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS; row < a.N; row += (int64_t)gridDim.x * ROWS) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-    int mine;
-    const Soft r = row_pass<T, THREADS>(x, a.V, mine, sh);
-    if (a.K) row_top<T, THREADS>(x, a.V, 0, a.K, mine, sh);
-    row_write<T, THREADS>(a, x, row, r, sh);
+    const int64_t t = target_of(a.target64, a.target32, row);
+    const bool has = t >= 0 && t < a.V;
+    const float given = has ? to_f(x[t]) : 0.f;  // the target's logit, on its way during the pass
+    Seen seen;
+    const Soft r = row_pass<T, THREADS>(x, a.V, seen, sh);
+    if (a.K) row_top<T, THREADS>(x, a.V, 0, a.K, seen, sh);
+    row_write<T, THREADS>(a, row, r, has, given, sh);
     row_sync<THREADS>();
   }
 }
 
-// Backward: a workgroup takes kBack elements of a row; p recomputed from the
-// row's maximum and sum.  The target's and the alternatives' own terms are
-// added by a rewrite of their elements behind a barrier.
-constexpr int kBack = 16384;
+// Backward: a workgroup takes a batch of its 256 threads from a row; p is
+// recomputed from the row's maximum and sum.  The target's and the
+// alternatives' own terms are added by a rewrite of their elements behind a
+// barrier, by the workgroup that wrote them.
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(TokenLogprobsBwd a, int parts) {
-  constexpr int N = Vec<T>::N;
+  constexpr int N = Vec<T>::N, SPAN = 256 * kUnroll;
   const int64_t items = (int64_t)a.N * parts;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t row = item / parts;
     const int part = (int)(item - row * parts);
-    const int lo = part * kBack, hi = min(a.C, lo + kBack);
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     T* dx = static_cast<T*>(a.dx) + row * a.C;
+    const int packs = a.V / N;
+    Batch<T, 256> v;
+    if (packs) v.load(x, part, packs);
     const int64_t t = target_of(a.target64, a.target32, row);
     const bool has = t >= 0 && t < a.V;
     const float m = a.stats[3 * row], s = a.stats[3 * row + 1];
@@ -272,30 +367,35 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(TokenLogprobsBwd a, i
     if (a.d_top)
       for (int k = 0; k < a.K; ++k) all += a.d_top[row * a.K + k];
     // dx_j = -p_j (all + dh (log p_j + entropy)) + own terms
-    const float inv = 1.f / s;
+    const float inv = 1.f / s, base = empty ? 0.f : m;
     const float ent = a.stats[3 * row + 2] - logf(s);
-    const float base = empty ? 0.f : m;
-    auto grad = [&](float v) -> float {
-      if (empty) return 0.f;
-      const float d = v - base, p = __builtin_amdgcn_exp2f(d * kLog2e) * inv;
+    auto grad = [&](float z) -> float {
+      const float d = z - base, p = __builtin_amdgcn_exp2f(d * kLog2e) * inv;
       float w = all;
       if (dh != 0.f) w = fmaf(dh, fmaxf(d, -1e4f) + ent, w);
-      return -p * w;
+      return empty ? 0.f : -p * w;
     };
-    for (int c = lo + threadIdx.x * N; c < hi; c += 256 * N) {
-      float f[N];
-      load_row<T, N>(x, c, a.V, -INFINITY, f);
 #pragma unroll
-      for (int k = 0; k < N; ++k) f[k] = c + k < a.V ? grad(f[k]) : 0.f;
-      store_row<T, N>(dx, c, hi, f);
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = part * SPAN + u * 256 + (int)threadIdx.x;
+      if (i < packs) {
+        Pack<T, N> o;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o.e[k] = from_f<T>(grad(to_f(v.v[u].e[k])));
+        store_pack<T, N>(dx + (int64_t)i * N, o);
+      }
     }
+    const int behind = packs * N;  // what is left of V, and the columns behind it: the last part's
+    if (part == parts - 1)
+      for (int j = behind + threadIdx.x; j < a.C; j += 256) dx[j] = from_f<T>(j < a.V ? grad(to_f(x[j])) : 0.f);
     __syncthreads();
+    const int lo = part * SPAN * N, hi = part == parts - 1 ? a.V : lo + SPAN * N;
     const int own = a.d_top ? a.K : 0;
+    // thread i: alternative i; the last one: the target, unless an alternative
+    // is the target (its thread adds both)
     for (int i = threadIdx.x; i <= own; i += 256) {
-      // thread i: alternative i; the last one: the target, unless an alternative
-      // is the target (its thread adds both)
-      int64_t j = i < own ? a.top_ids[row * a.K + i] : (has ? t : -1);
-      if (j < lo || j >= hi || j >= a.V || empty) continue;
+      const int64_t j = i < own ? a.top_ids[row * a.K + i] : (has ? t : -1);
+      if (j < lo || j >= hi || empty) continue;
       float extra = i < own ? a.d_top[row * a.K + i] : dl;
       bool mine = true;
       for (int k = 0; k < own; ++k)
@@ -317,7 +417,7 @@ void fwd_typed(const TokenLogprobs& a, hipStream_t s) {
   if (a.V <= 2048) {
     const int64_t want = ((int64_t)a.N + 3) / 4;
     logprobs_kernel<T, 64><<<(unsigned)(want < cap ? want : cap), 256, 0, s>>>(a);
-  } else if (a.V <= 16384) {
+  } else if (a.N >= 1024) {
     logprobs_kernel<T, 256><<<(unsigned)(a.N < cap ? a.N : cap), 256, 0, s>>>(a);
   } else {
     logprobs_kernel<T, 1024><<<(unsigned)(a.N < cap ? a.N : cap), 1024, 0, s>>>(a);
@@ -325,7 +425,7 @@ void fwd_typed(const TokenLogprobs& a, hipStream_t s) {
 }
 template <typename T>
 void bwd_typed(const TokenLogprobsBwd& a, hipStream_t s) {
-  const int parts = (a.C + kBack - 1) / kBack;
+  const int packs = a.V / Vec<T>::N, span = 256 * kUnroll, parts = packs > span ? (packs + span - 1) / span : 1;
   const int64_t items = (int64_t)a.N * parts, cap = 1 << 20;
   logprobs_bwd_kernel<T><<<(unsigned)(items < cap ? items : cap), 256, 0, s>>>(a, parts);
 }
