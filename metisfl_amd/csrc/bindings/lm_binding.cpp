@@ -31,15 +31,33 @@ int elem_type(const Tensor& t, const char* nm) {
   }
 }
 
-// [rows][cols] with the columns one element apart -> the row stride
-int64_t rows_stride(const Tensor& t, const char* nm) {
-  TORCH_CHECK(t.is_cuda(), nm, " must be a device tensor");
-  TORCH_CHECK(t.dim() == 2, nm, " must have two dimensions");
-  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, nm, " must have its columns one element apart");
-  TORCH_CHECK(t.size(0) < std::numeric_limits<int>::max() && t.size(1) < std::numeric_limits<int>::max() - 65536, nm,
-              " has too many rows or columns");
-  return t.size(0) > 1 ? t.stride(0) : t.size(1);
-}
+// A tensor of any dimensions as rows of its last one: columns one element
+// apart, rows a fixed stride apart (a copy where the strides allow no such view).
+struct Rows {
+  Tensor keep;
+  void* p = nullptr;
+  int64_t rows = 1, cols = 0, stride = 0;
+
+  Rows(const Tensor& t, const char* nm) : keep(t) {
+    TORCH_CHECK(t.is_cuda(), nm, " must be a device tensor");
+    TORCH_CHECK_VALUE(t.dim() > 0, nm, " must have at least one dimension");
+    const int64_t d = t.dim();
+    cols = t.size(d - 1);
+    for (int64_t i = 0; i + 1 < d; ++i) rows *= t.size(i);
+    TORCH_CHECK(rows < std::numeric_limits<int>::max() && cols < std::numeric_limits<int>::max() - 65536, nm,
+                " has too many rows or columns");
+    if (t.is_contiguous()) {
+      stride = cols;
+    } else if (d == 2 && (t.stride(1) == 1 || cols == 1)) {
+      stride = t.stride(0);
+    } else {
+      if (cols > 1 && t.stride(d - 1) != 1) keep = t.contiguous();
+      if (d != 2) keep = keep.reshape({rows, cols});
+      stride = keep.dim() == 2 ? keep.stride(0) : cols;
+    }
+    p = keep.data_ptr();
+  }
+};
 
 void same_device(const Tensor& t, const Tensor& x, const char* nm) {
   TORCH_CHECK(t.device() == x.device(), nm, " is on ", t.device(), ", expected ", x.device());
@@ -58,32 +76,42 @@ int param_type(const Tensor& p, const Tensor& x, int64_t H, const char* nm) {
   return t;
 }
 
+c10::IntArrayRef lead_of(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
+
+void norm_weights(const Tensor& x, int64_t H, const OptTensor& gamma, const OptTensor& beta) {
+  TORCH_CHECK_VALUE(H > 0, "x has rows of no elements");
+  TORCH_CHECK_VALUE(!given(beta) || given(gamma), "beta without gamma");
+  for (const auto* p : {&gamma, &beta})
+    TORCH_CHECK_VALUE(!given(*p) || ((*p)->dim() == 1 && (*p)->size(0) == H), p == &gamma ? "gamma" : "beta",
+                      " has shape ", (*p)->sizes(), ", expected (", H, ")");
+}
+
 std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x, const OptTensor& gamma, const OptTensor& beta,
                                                   double eps) {
-  const int64_t ldx = rows_stride(x, "x"), M = x.size(0), H = x.size(1);
+  const Rows r(x, "x");
+  norm_weights(x, r.cols, gamma, beta);
   c10::DeviceGuard guard(x.device());
   mfl::LayerNormFwd a{};
   a.type = elem_type(x, "x");
-  TORCH_CHECK(H > 0, "x has rows of no elements");
   a.param_type = mfl::ELEM_F32;
-  if (given(gamma)) a.param_type = param_type(*gamma, x, H, "gamma");
-  if (given(beta)) {
-    TORCH_CHECK(given(gamma), "beta without gamma");
-    TORCH_CHECK(param_type(*beta, x, H, "beta") == a.param_type, "gamma and beta must have the same type");
+  if (given(gamma)) {
+    a.param_type = param_type(*gamma, x, r.cols, "gamma");
+    a.gamma = gamma->data_ptr();
   }
-  Tensor y = torch::empty({M, H}, x.options());
-  Tensor mean = torch::empty({M}, x.options().dtype(torch::kFloat32));
-  Tensor rstd = torch::empty({M}, x.options().dtype(torch::kFloat32));
-  if (M == 0) return {y, mean, rstd};
-  a.x = x.data_ptr();
-  a.gamma = given(gamma) ? gamma->data_ptr() : nullptr;
-  a.beta = given(beta) ? beta->data_ptr() : nullptr;
+  if (given(beta)) {
+    TORCH_CHECK(param_type(*beta, x, r.cols, "beta") == a.param_type, "gamma and beta must have the same type");
+    a.beta = beta->data_ptr();
+  }
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  Tensor y = at::empty(x.sizes(), x.options()), mean = at::empty(lead_of(x), f32), rstd = at::empty(lead_of(x), f32);
+  if (r.rows == 0) return {y, mean, rstd};
+  a.x = r.p;
   a.y = y.data_ptr();
   a.mean = mean.data_ptr<float>();
   a.rstd = rstd.data_ptr<float>();
-  a.ldx = ldx;
-  a.M = (int)M;
-  a.H = (int)H;
+  a.ldx = r.stride;
+  a.M = (int)r.rows;
+  a.H = (int)r.cols;
   a.eps = (float)eps;
   mfl::launch_layer_norm_fwd(a, stream_of(x));
   C10_HIP_KERNEL_LAUNCH_CHECK();
@@ -92,36 +120,37 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x, const OptTens
 
 std::tuple<Tensor, OptTensor, OptTensor> layer_norm_bwd(const Tensor& dy, const Tensor& x, const Tensor& mean,
                                                         const Tensor& rstd, const OptTensor& gamma) {
-  const int64_t ldx = rows_stride(x, "x"), lddy = rows_stride(dy, "dy"), M = x.size(0), H = x.size(1);
+  TORCH_CHECK_VALUE(dy.sizes() == x.sizes(), "dy has shape ", dy.sizes(), ", expected ", x.sizes());
+  const Rows r(x, "x"), d(dy, "dy");
+  norm_weights(x, r.cols, gamma, c10::nullopt);
   c10::DeviceGuard guard(x.device());
   mfl::LayerNormBwd a{};
   a.type = elem_type(x, "x");
-  TORCH_CHECK(H > 0, "x has rows of no elements");
   same_device(dy, x, "dy");
-  TORCH_CHECK(dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes(), "dy must have x's type and shape");
-  vector_of(mean, x, torch::kFloat32, M, "mean");
-  vector_of(rstd, x, torch::kFloat32, M, "rstd");
-  a.param_type = given(gamma) ? param_type(*gamma, x, H, "gamma") : mfl::ELEM_F32;
-  Tensor dx = torch::empty({M, H}, x.options());
+  TORCH_CHECK(dy.scalar_type() == x.scalar_type(), "dy must have x's type and shape");
+  vector_of(mean, x, torch::kFloat32, r.rows, "mean");
+  vector_of(rstd, x, torch::kFloat32, r.rows, "rstd");
+  a.param_type = given(gamma) ? param_type(*gamma, x, r.cols, "gamma") : mfl::ELEM_F32;
+  Tensor dx = at::empty(x.sizes(), x.options());
   OptTensor dgamma, dbeta;
   if (given(gamma)) {
-    dgamma = M ? torch::empty({H}, gamma->options()) : torch::zeros({H}, gamma->options());
-    dbeta = M ? torch::empty({H}, gamma->options()) : torch::zeros({H}, gamma->options());
+    dgamma = r.rows ? at::empty({r.cols}, gamma->options()) : at::zeros({r.cols}, gamma->options());
+    dbeta = r.rows ? at::empty({r.cols}, gamma->options()) : at::zeros({r.cols}, gamma->options());
   }
-  if (M == 0) return {dx, dgamma, dbeta};
+  if (r.rows == 0) return {dx, dgamma, dbeta};
   Tensor part;  // the workgroups' partial sums, from the allocator of the current stream (or of a capture)
-  a.dy = dy.data_ptr();
-  a.x = x.data_ptr();
+  a.dy = d.p;
+  a.x = r.p;
   a.mean = mean.data_ptr<float>();
   a.rstd = rstd.data_ptr<float>();
   a.dx = dx.data_ptr();
-  a.ldx = ldx;
-  a.lddy = lddy;
-  a.M = (int)M;
-  a.H = (int)H;
+  a.ldx = r.stride;
+  a.lddy = d.stride;
+  a.M = (int)r.rows;
+  a.H = (int)r.cols;
   if (given(gamma)) {
-    const int64_t G = mfl::layer_norm_bwd_blocks((int)M, (int)H, a.type);
-    part = torch::empty({G * 2 * H}, x.options().dtype(torch::kFloat32));
+    const int64_t G = mfl::layer_norm_bwd_blocks(a.M, a.H, a.type);
+    part = at::empty({G * 2 * r.cols}, x.options().dtype(torch::kFloat32));
     a.part = part.data_ptr<float>();
     a.gamma = gamma->data_ptr();
     a.dgamma = dgamma->data_ptr();
@@ -132,84 +161,112 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_bwd(const Tensor& dy, const 
   return {dx, dgamma, dbeta};
 }
 
-// targets of any whole type the kernels read
-void set_target(const Tensor& target, const Tensor& x, int64_t N, const int64_t*& t64, const int32_t*& t32) {
-  same_device(target, x, "targets");
-  TORCH_CHECK(target.is_contiguous() && target.numel() == N, "targets must be contiguous, one for each row");
-  if (target.scalar_type() == torch::kInt64) t64 = target.data_ptr<int64_t>();
-  else if (target.scalar_type() == torch::kInt32) t32 = target.data_ptr<int32_t>();
-  else TORCH_CHECK(false, "targets must be int64 or int32, got ", target.scalar_type());
+// The targets of rows of logits: one whole number each.
+struct Targets {
+  Tensor keep;
+  const int64_t* t64 = nullptr;
+  const int32_t* t32 = nullptr;
+
+  Targets(const Tensor& t, const Tensor& x) : keep(t) {
+    TORCH_CHECK_VALUE(t.sizes() == lead_of(x), "targets have shape ", t.sizes(), ", expected ", lead_of(x));
+    TORCH_CHECK_TYPE(t.scalar_type() == torch::kInt64 || t.scalar_type() == torch::kInt32,
+                     "targets must be int64 or int32, got ", t.scalar_type());
+    same_device(t, x, "targets");
+    if (!t.is_contiguous()) keep = t.contiguous();
+    if (t.scalar_type() == torch::kInt64) t64 = keep.data_ptr<int64_t>();
+    else t32 = keep.data_ptr<int32_t>();
+  }
+};
+
+int64_t vocab_of(const Rows& r, const c10::optional<int64_t>& vocab) {
+  const int64_t V = vocab.value_or(r.cols);
+  TORCH_CHECK_VALUE(V > 0 && V <= r.cols, "vocab must be between 1 and the logits' ", r.cols, " columns, got ", V);
+  return V;
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_fwd(const Tensor& x, const Tensor& target,
-                                                                      int64_t V, int64_t K) {
-  const int64_t ldx = rows_stride(x, "logits"), N = x.size(0);
+                                                                      int64_t K, c10::optional<int64_t> vocab) {
+  const Rows r(x, "logits");
+  const int64_t V = vocab_of(r, vocab);
+  TORCH_CHECK_VALUE(K >= 0 && K <= mfl::kTopMax && K <= V, "top_k must be between 0 and ", mfl::kTopMax,
+                    " and at most vocab, got ", K);
+  const Targets t(target, x);
   c10::DeviceGuard guard(x.device());
   mfl::TokenLogprobs a{};
   a.type = elem_type(x, "logits");
-  TORCH_CHECK(V > 0 && V <= x.size(1), "vocab must be between 1 and the logits' ", x.size(1), " columns, got ", V);
-  TORCH_CHECK(K >= 0 && K <= mfl::kTopMax && K <= V, "top_k must be between 0 and ", mfl::kTopMax,
-              " and at most vocab, got ", K);
-  set_target(target, x, N, a.target64, a.target32);
   const auto f32 = x.options().dtype(torch::kFloat32);
-  Tensor logp = torch::empty({N}, f32), entropy = torch::empty({N}, f32), stats = torch::empty({N, 3}, f32);
-  Tensor top = torch::empty({N, K}, f32), ids = torch::empty({N, K}, x.options().dtype(torch::kInt64));
-  if (N == 0) return {logp, entropy, stats, top, ids};
-  Tensor work;
-  const size_t bytes = mfl::token_logprobs_workspace((int)N, (int)V, (int)K, a.type);
-  if (bytes) {
-    work = torch::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8));
+  auto shape = lead_of(x).vec();
+  Tensor logp = at::empty(shape, f32), entropy = at::empty(shape, f32);
+  shape.push_back(3);
+  Tensor stats = at::empty(shape, f32);
+  shape.back() = K;
+  Tensor top = at::empty(shape, f32), ids = at::empty(shape, x.options().dtype(torch::kInt64));
+  if (r.rows == 0) return {logp, entropy, top, ids, stats};
+  Tensor work;  // parts of split rows, from the allocator of the current stream (or of a capture)
+  if (const size_t bytes = mfl::token_logprobs_workspace((int)r.rows, (int)V, (int)K, a.type)) {
+    work = at::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8));
     a.work = work.data_ptr();
   }
-  a.x = x.data_ptr();
+  a.x = r.p;
+  a.target64 = t.t64;
+  a.target32 = t.t32;
   a.logp = logp.data_ptr<float>();
   a.entropy = entropy.data_ptr<float>();
   a.stats = stats.data_ptr<float>();
   a.top_logp = top.data_ptr<float>();
   a.top_ids = ids.data_ptr<int64_t>();
-  a.ldx = ldx;
-  a.N = (int)N;
+  a.ldx = r.stride;
+  a.N = (int)r.rows;
   a.V = (int)V;
   a.K = (int)K;
   mfl::launch_token_logprobs(a, stream_of(x));
   C10_HIP_KERNEL_LAUNCH_CHECK();
-  return {logp, entropy, stats, top, ids};
+  return {logp, entropy, top, ids, stats};
 }
 
 Tensor token_logprobs_bwd(const Tensor& x, const Tensor& target, const Tensor& stats, const OptTensor& d_logp,
                           const OptTensor& d_entropy, const OptTensor& d_top, const OptTensor& top_ids,
-                          int64_t V) {
-  const int64_t ldx = rows_stride(x, "logits"), N = x.size(0), C = x.size(1);
+                          c10::optional<int64_t> vocab) {
+  const Rows r(x, "logits");
+  const int64_t V = vocab_of(r, vocab), N = r.rows;
+  const Targets t(target, x);
+  const auto lead = lead_of(x);
+  auto rows_by = [&](const Tensor& v) { return v.dim() == x.dim() && lead_of(v) == lead; };
+  TORCH_CHECK_VALUE(rows_by(stats) && stats.size(-1) == 3, "stats have shape ", stats.sizes(),
+                    ", expected the rows' shape and 3");
+  for (const auto* d : {&d_logp, &d_entropy})
+    TORCH_CHECK_VALUE(!given(*d) || (*d)->sizes() == lead, d == &d_logp ? "d_logp" : "d_entropy", " has shape ",
+                      (*d)->sizes(), ", expected ", lead);
+  TORCH_CHECK_VALUE(!given(d_top) || (given(top_ids) && rows_by(*d_top) && d_top->sizes() == top_ids->sizes()),
+                    "d_top needs top_ids, both with the rows' shape and one column for each alternative");
   c10::DeviceGuard guard(x.device());
   mfl::TokenLogprobsBwd a{};
   a.type = elem_type(x, "logits");
-  TORCH_CHECK(V > 0 && V <= C, "vocab must be between 1 and the logits' ", C, " columns, got ", V);
-  set_target(target, x, N, a.target64, a.target32);
-  vector_of(stats, x, torch::kFloat32, 3 * N, "stats");
-  if (given(d_logp)) vector_of(*d_logp, x, torch::kFloat32, N, "d_logp");
-  if (given(d_entropy)) vector_of(*d_entropy, x, torch::kFloat32, N, "d_entropy");
-  if (given(d_top)) {
-    TORCH_CHECK(given(top_ids) && d_top->dim() == 2, "d_top needs top_ids and two dimensions");
-    a.K = (int)d_top->size(1);
-    TORCH_CHECK(d_top->size(1) <= mfl::kTopMax, "d_top has more than ", mfl::kTopMax, " columns");
-    vector_of(*d_top, x, torch::kFloat32, N * a.K, "d_top");
-    vector_of(*top_ids, x, torch::kInt64, N * a.K, "top_ids");
+  std::vector<Tensor> keep;  // contiguous copies (the gradient of a sum is an expanded number)
+  auto whole = [&](const Tensor& v, torch::ScalarType dt, int64_t n, const char* nm) {
+    keep.push_back(v.contiguous());
+    vector_of(keep.back(), x, dt, n, nm);
+    return keep.back().data_ptr();
+  };
+  a.stats = static_cast<const float*>(whole(stats, torch::kFloat32, 3 * N, "stats"));
+  if (given(d_logp)) a.d_logp = static_cast<const float*>(whole(*d_logp, torch::kFloat32, N, "d_logp"));
+  if (given(d_entropy)) a.d_entropy = static_cast<const float*>(whole(*d_entropy, torch::kFloat32, N, "d_entropy"));
+  if (given(d_top) && d_top->size(-1)) {
+    TORCH_CHECK_VALUE(d_top->size(-1) <= mfl::kTopMax, "d_top has more than ", mfl::kTopMax, " columns");
+    a.K = (int)d_top->size(-1);
+    a.d_top = static_cast<const float*>(whole(*d_top, torch::kFloat32, N * a.K, "d_top"));
+    a.top_ids = static_cast<const int64_t*>(whole(*top_ids, torch::kInt64, N * a.K, "top_ids"));
   }
-  Tensor dx = torch::empty({N, C}, x.options());
+  Tensor dx = at::empty(x.sizes(), x.options());
   if (N == 0) return dx;
-  a.x = x.data_ptr();
-  a.stats = stats.data_ptr<float>();
-  a.d_logp = given(d_logp) ? d_logp->data_ptr<float>() : nullptr;
-  a.d_entropy = given(d_entropy) ? d_entropy->data_ptr<float>() : nullptr;
-  if (given(d_top) && a.K) {
-    a.d_top = d_top->data_ptr<float>();
-    a.top_ids = top_ids->data_ptr<int64_t>();
-  }
+  a.x = r.p;
+  a.target64 = t.t64;
+  a.target32 = t.t32;
   a.dx = dx.data_ptr();
-  a.ldx = ldx;
+  a.ldx = r.stride;
   a.N = (int)N;
   a.V = (int)V;
-  a.C = (int)C;
+  a.C = (int)r.cols;
   mfl::launch_token_logprobs_bwd(a, stream_of(x));
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return dx;

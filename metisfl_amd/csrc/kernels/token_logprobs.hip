@@ -27,6 +27,7 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kList = 1024;  // candidates of a row (LDS)
+constexpr int kSplitRows = 128, kSplitWidth = 32768, kSplitGroups = 512;  // see part_span
 
 // Running maximum m, sum of exp(x - m) and sum of exp(x - m) (x - m) log2 e.
 // exp(x - m) = exp2(x L - fl(m L)) with L = log2 e is one fused multiply-add
@@ -105,7 +106,7 @@ template <int THREADS>
 struct RowShared {
   float m[16], s[16], t[16];
   float group[64];
-  int count;
+  int bound, count;
   uint64_t best[16], top[kTopMax], list[THREADS > 64 ? kList : 256];
 };
 
@@ -168,18 +169,21 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, Seen seen, Row
   }
   if constexpr (GROUP > 1) {
     if (tid % GROUP == 0) sh.group[tid / GROUP] = g;
-    if (tid == 0) sh.count = 0;
-    row_sync<THREADS>();
+    __syncthreads();
     g = sh.group[tid & 63];
-  } else if (tid == 0) {
-    sh.count = 0;
   }
-  int above = 0;  // groups above this lane's
+  if (tid < 64) {  // (the first wave)
+    int above = 0;  // groups above this lane's
 #pragma unroll
-  for (int j = 0; j < 64; ++j) above += lane_of(g, j) > g;
-  const float least = -max64(above < K ? -g : -INFINITY);
-  const int bound = order_of(least);
+    for (int j = 0; j < 64; ++j) above += lane_of(g, j) > g;
+    const float least = -max64(above < K ? -g : -INFINITY);
+    if (tid == 0) {
+      sh.bound = order_of(least);
+      sh.count = 0;
+    }
+  }
   row_sync<THREADS>();
+  const int bound = sh.bound;
   // threads that saw an element of that size list theirs
   const int packs = n / N, batches = (packs + THREADS * kUnroll - 1) / (THREADS * kUnroll);
   if (packs && order_of(seen.largest) >= bound) {
@@ -341,6 +345,79 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void logprobs_kernel
   }
 }
 
+// Few long rows: a workgroup to each part of a row (a whole number of batches)
+// writes the part's sums and its K largest; a wave to each row joins them.
+struct PartSums {
+  float m, s, t, unused;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void logprobs_part_kernel(TokenLogprobs a, int span) {
+  __shared__ RowShared<256> sh;
+  const int part = blockIdx.x, parts = gridDim.x;
+  const int64_t row = blockIdx.y;
+  const int lo = part * span, n = min(span, a.V - lo);
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx + lo;
+  Seen seen;
+  const Soft r = row_pass<T, 256>(x, n, seen, sh);
+  const int K = min(a.K, n);
+  if (K) row_top<T, 256>(x, n, (uint32_t)lo, K, seen, sh);
+  PartSums* sums = static_cast<PartSums*>(a.work);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(sums + (int64_t)a.N * parts);
+  if (threadIdx.x == 0) sums[row * parts + part] = {r.m, r.s, r.t, 0.f};
+  if ((int)threadIdx.x < a.K) keys[(row * parts + part) * a.K + threadIdx.x] = (int)threadIdx.x < K ? sh.top[threadIdx.x] : 0;
+}
+template <typename T>
+__global__ __launch_bounds__(64) void logprobs_join_kernel(TokenLogprobs a, int parts) {
+  __shared__ RowShared<64> sh;
+  __shared__ uint64_t lists[64 * kTopMax];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const PartSums* sums = static_cast<const PartSums*>(a.work);
+  const uint64_t* keys = reinterpret_cast<const uint64_t*>(sums + (int64_t)a.N * parts) + row * parts * a.K;
+  for (int i = lane; i < parts * a.K; i += 64) lists[i] = keys[i];
+  const int64_t t = target_of(a.target64, a.target32, row);
+  const bool has = t >= 0 && t < a.V;
+  const float given = has ? to_f(x[t]) : 0.f;
+  Soft r = {-INFINITY, 0.f, 0.f};
+  if (lane < parts) {
+    const PartSums p = sums[row * parts + lane];
+    r = {p.m, p.s, p.t * kLog2e};
+  }
+  soft_raise(r, max64(r.m));
+  r.s = lane_sum<64>(r.s);
+  r.t = lane_sum<64>(r.t) * kLn2;
+  row_sync<64>();
+  // each part's list is in order, and so are the parts' ids: the first lane
+  // with the largest head has the next alternative
+  int next = 1;
+  uint64_t head = lane < parts && a.K ? lists[lane * a.K] : 0;
+  for (int k = 0; k < a.K; ++k) {
+    const uint32_t mine = (uint32_t)(head >> 32);  // (0 behind a list's end, below every logit's)
+    uint32_t best = mine;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, o, 64));
+    if (lane == __ffsll((unsigned long long)__ballot(mine == best)) - 1) {
+      sh.top[k] = head;
+      head = next < a.K ? lists[lane * a.K + next] : 0;
+      ++next;
+    }
+  }
+  row_sync<64>();
+  row_write<T, 64>(a, row, r, has, given, sh);
+}
+// Elements of a part, or 0 for rows that are not split: only rows that leave
+// most of the chip idle are, into batches of 256 threads, at most 64.
+int part_span(int N, int V, int type) {
+  const int batch = 256 * kUnroll * (type == ELEM_F32 ? 4 : 8);
+  if (N > kSplitRows || V < kSplitWidth) return 0;
+  const int64_t batches = ((int64_t)V + batch - 1) / batch;
+  int64_t parts = kSplitGroups / N;
+  parts = parts < 64 ? parts : 64;
+  parts = parts < batches ? parts : batches;
+  return (int)((batches + parts - 1) / parts * batch);
+}
+
 // Backward: a workgroup takes a batch of its 256 threads from a row; p is
 // recomputed from the row's maximum and sum.  The target's and the
 // alternatives' own terms are added by a rewrite of their elements behind a
@@ -414,6 +491,12 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(TokenLogprobsBwd a, i
 template <typename T>
 void fwd_typed(const TokenLogprobs& a, hipStream_t s) {
   const int64_t cap = 1 << 20;
+  if (const int span = part_span(a.N, a.V, a.type)) {
+    const int parts = (a.V + span - 1) / span;
+    logprobs_part_kernel<T><<<dim3(parts, a.N), 256, 0, s>>>(a, span);
+    logprobs_join_kernel<T><<<a.N, 64, 0, s>>>(a, parts);
+    return;
+  }
   if (a.V <= 2048) {
     const int64_t want = ((int64_t)a.N + 3) / 4;
     logprobs_kernel<T, 64><<<(unsigned)(want < cap ? want : cap), 256, 0, s>>>(a);
@@ -432,7 +515,10 @@ void bwd_typed(const TokenLogprobsBwd& a, hipStream_t s) {
 
 }  // namespace
 
-size_t token_logprobs_workspace(int, int, int, int) { return 0; }
+size_t token_logprobs_workspace(int N, int V, int K, int type) {
+  const int span = part_span(N, V, type);
+  return span ? (size_t)N * ((V + span - 1) / span) * (sizeof(PartSums) + (size_t)K * sizeof(uint64_t)) : 0;
+}
 
 void launch_token_logprobs(const TokenLogprobs& a, hipStream_t s) {
   if (a.type == ELEM_F32) fwd_typed<float>(a, s);

@@ -24,13 +24,9 @@ TOP_MAX = 32
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as [rows][last dimension], columns one element apart (a view where the strides allow it)."""
+    """``t`` as [rows][last dimension]."""
     if t.dim() == 0:
         raise ValueError("a tensor with at least one dimension is needed")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        t = t.contiguous()
-    if t.dim() == 2:
-        return t
     rows = 1
     for n in t.shape[:-1]:
         rows *= n
@@ -57,21 +53,19 @@ def layer_norm_fwd(x, gamma=None, beta=None, eps: float = 1e-5):
     y = (x - mean) * rstd * gamma + beta in x's type, mean and rstd float32,
     one for each row.  ``gamma`` / ``beta`` are float32 or of x's type;
     without ``gamma`` the norm has no weights."""
-    _check_norm(x, gamma, beta)
-    r = _rows(x)
     if x.is_cuda:
-        y, mean, rstd = ops().layer_norm_fwd(r, gamma, beta, eps)
-    else:
-        w = _wide(r)
-        mean = w.mean(1)
-        d = w - mean[:, None]
-        rstd = torch.rsqrt((d * d).mean(1) + eps)
-        y = d * rstd[:, None]
-        if gamma is not None:
-            y = y * gamma
-        if beta is not None:
-            y = y + beta
-        y = y.to(x.dtype)
+        return ops().layer_norm_fwd(x, gamma, beta, eps)
+    _check_norm(x, gamma, beta)
+    w = _wide(_rows(x))
+    mean = w.mean(1)
+    d = w - mean[:, None]
+    rstd = torch.rsqrt((d * d).mean(1) + eps)
+    y = d * rstd[:, None]
+    if gamma is not None:
+        y = y * gamma
+    if beta is not None:
+        y = y + beta
+    y = y.to(x.dtype)
     return y.view(x.shape), mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
 
 
@@ -79,15 +73,13 @@ def layer_norm_bwd(dy, x, mean, rstd, gamma=None):
     """``(dx, dgamma, dbeta)`` from the forward's input and statistics; the
     weights' gradients in gamma's type, None without ``gamma``.  They are
     sums in a fixed order (no atomics)."""
+    if x.is_cuda:
+        return ops().layer_norm_bwd(dy, x, mean, rstd, gamma)
     _check_norm(x, gamma, None)
     if dy.shape != x.shape:
         raise ValueError(f"dy has shape {tuple(dy.shape)}, expected {tuple(x.shape)}")
-    r = _rows(x)
-    if x.is_cuda:
-        dx, dgamma, dbeta = ops().layer_norm_bwd(_rows(dy), r, mean.reshape(-1), rstd.reshape(-1), gamma)
-        return dx.view(x.shape), dgamma, dbeta
     d = _wide(_rows(dy))
-    xh = (_wide(r) - mean.reshape(-1, 1)) * rstd.reshape(-1, 1)
+    xh = (_wide(_rows(x)) - mean.reshape(-1, 1)) * rstd.reshape(-1, 1)
     u = d if gamma is None else d * gamma
     dx = rstd.reshape(-1, 1) * (u - u.mean(1, keepdim=True) - xh * (u * xh).mean(1, keepdim=True))
     dx = dx.to(x.dtype).view(x.shape)
@@ -163,14 +155,11 @@ def token_logprobs_fwd(logits, targets, top_k: int = 0, vocab: int | None = None
     row of nothing but -inf gives logp and top_logp -inf and entropy 0; NaN
     or +inf in a row makes its results NaN, and NaN ranks lowest among the
     alternatives."""
+    if logits.is_cuda:
+        return TokenLogprobs(*ops().token_logprobs_fwd(logits, targets, top_k, vocab))
     vocab = _check_logits(logits, targets, vocab, top_k)
     lead = logits.shape[:-1]
-    r, t = _rows(logits), targets.reshape(-1).contiguous()
-    if logits.is_cuda:
-        logp, entropy, stats, top, ids = ops().token_logprobs_fwd(r, t, vocab, top_k)
-        return TokenLogprobs(logp.view(lead), entropy.view(lead), top.view(*lead, top_k), ids.view(*lead, top_k),
-                             stats.view(*lead, 3))
-    z, t = _wide(r[:, :vocab]), t.long()
+    z, t = _wide(_rows(logits)[:, :vocab]), targets.reshape(-1).long()
     top, e, s, d, empty = _soft_ref(z)
     logs = torch.log(s)
     has = (t >= 0) & (t < vocab)
@@ -191,6 +180,8 @@ def token_logprobs_bwd(logits, targets, stats, d_logp=None, d_entropy=None, d_to
     """Gradient of the logits in their type (columns from ``vocab`` on zero)
     from the forward's ``stats`` and the gradients of its results, each float32
     or None; ``d_top`` needs the forward's ``top_ids``."""
+    if logits.is_cuda:
+        return ops().token_logprobs_bwd(logits, targets, stats, d_logp, d_entropy, d_top, top_ids, vocab)
     vocab = _check_logits(logits, targets, vocab)
     lead = tuple(logits.shape[:-1])
     if tuple(stats.shape) != lead + (3,):
@@ -200,13 +191,10 @@ def token_logprobs_bwd(logits, targets, stats, d_logp=None, d_entropy=None, d_to
             raise ValueError(f"{nm} has shape {tuple(v.shape)}, expected {lead}")
     if d_top is not None and (top_ids is None or d_top.shape != top_ids.shape or tuple(d_top.shape[:-1]) != lead):
         raise ValueError("d_top needs top_ids, both with the rows' shape and one column for each alternative")
-    r, t = _rows(logits), targets.reshape(-1).contiguous()
+    r, t = _rows(logits), targets.reshape(-1)
     n = r.shape[0]
-    flat = lambda v: None if v is None else v.reshape(-1).contiguous()  # noqa: E731
-    flat2 = lambda v: None if v is None else v.reshape(n, v.shape[-1]).contiguous()  # noqa: E731
-    if logits.is_cuda:
-        return ops().token_logprobs_bwd(r, t, flat2(stats), flat(d_logp), flat(d_entropy), flat2(d_top),
-                                        flat2(top_ids), vocab).view(logits.shape)
+    flat = lambda v: None if v is None else v.reshape(-1)  # noqa: E731
+    flat2 = lambda v: None if v is None else v.reshape(n, v.shape[-1])  # noqa: E731
     z, t, stats = _wide(r[:, :vocab]), t.long(), flat2(stats)
     m, s, entropy = stats[:, :1], stats[:, 1:2], stats[:, 2:]
     empty = (m == float("-inf")) & (s == 0)
