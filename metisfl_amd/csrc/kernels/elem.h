@@ -50,32 +50,6 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& v) {
   __builtin_memcpy(p, &v, sizeof(v));
 }
 
-// Elements c .. c + N - 1 of a row of H (those at or behind H: `fill`).
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T* row, int c, int H, float fill, float* f) {
-  if (c + N <= H) {
-    const Pack<T, N> v = load_pack<T, N>(row + c);
-#pragma unroll
-    for (int k = 0; k < N; ++k) f[k] = to_f(v.e[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k) f[k] = c + k < H ? to_f(row[c + k]) : fill;
-  }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_row(T* row, int c, int H, const float* f) {
-  if (c + N <= H) {
-    Pack<T, N> v;
-#pragma unroll
-    for (int k = 0; k < N; ++k) v.e[k] = from_f<T>(f[k]);
-    store_pack<T, N>(row + c, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (c + k < H) row[c + k] = from_f<T>(f[k]);
-  }
-}
-
 // Reductions over a wave's rows of 16 lanes by DPP rotations (every lane gets
 // the result; a rotation costs a VALU instruction where a shuffle goes through
 // LDS), and over all 64 lanes by four lane reads more.  The lanes of a row (of

@@ -18,12 +18,17 @@
 #include "kernels/elem.h"
 #include "kernels/lm.h"
 
+#include <type_traits>
+
 namespace mfl {
 namespace {
 
+// Which of a workgroup's rows a thread works on: a scalar where a wave has one row.
 template <int LANES>
-constexpr int block_of() {
-  return LANES > 256 ? LANES : 256;
+__device__ __forceinline__ int row_group() {
+  const int g = threadIdx.x / LANES;
+  if constexpr (LANES >= 64) return __builtin_amdgcn_readfirstlane(g);
+  return g;
 }
 
 // Sums of a and b over the LANES threads of a row; with more than one wave
@@ -41,31 +46,86 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* buf) {
       buf[16 + w] = b;
     }
     __syncthreads();
-    a = b = 0.f;
+    if constexpr (W == 16) {
+      a = sum16(buf[threadIdx.x & 15]);
+      b = sum16(buf[16 + (threadIdx.x & 15)]);
+    } else {
+      a = b = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      a += buf[i];
-      b += buf[16 + i];
+      for (int i = 0; i < W; ++i) {
+        a += buf[i];
+        b += buf[16 + i];
+      }
     }
   }
 }
 
-template <typename T, typename P, int LANES, int VPL>
-__global__ __launch_bounds__(block_of<LANES>()) void ln_fwd_kernel(LayerNormFwd a) {
-  constexpr int N = Vec<T>::N, ROWS = block_of<LANES>() / LANES;
+// The packs of N columns that a lane has of every row: pack i starts at
+// column c[i]; one that would end behind the row (or lie there) is moved back
+// to end with it, and its first skip[i] elements, another lane's, count for
+// nothing.  So every load is whole and in the row, whatever its width (>= N).
+template <int LANES, int VPL, int N>
+struct Columns {
+  int c[VPL], skip[VPL];
+  // shapes hold a row in no more packs than needed: the first ones are whole
+  static constexpr bool whole(int i) { return VPL > 1 && i < VPL / 2; }
+  __device__ __forceinline__ Columns(int lane, int H) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int at = (i * LANES + lane) * N;
+      c[i] = whole(i) || at <= H - N ? at : H - N;
+      skip[i] = at - c[i];
+    }
+  }
+  __device__ __forceinline__ bool has(int i, int k) const { return whole(i) || k >= skip[i]; }
+  __device__ __forceinline__ bool full(int i) const { return whole(i) || skip[i] == 0; }
+  __device__ __forceinline__ bool any(int i) const { return whole(i) || skip[i] < N; }
+};
+template <typename T, int LANES, int VPL, int N>
+__device__ __forceinline__ void load_packs(const T* row, const Columns<LANES, VPL, N>& at, Pack<T, N> (&v)[VPL]) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) v[i] = load_pack<T, N>(row + at.c[i]);
+}
+template <typename P, int LANES, int VPL, int N>
+__device__ __forceinline__ void load_weights(const void* p, const Columns<LANES, VPL, N>& at, float none,
+                                             float (&w)[VPL][N]) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    Pack<P, N> v;
+    if (p) v = load_pack<P, N>(static_cast<const P*>(p) + at.c[i]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) w[i][k] = p ? to_f(v.e[k]) : none;
+  }
+}
+
+// A workgroup's rows: its BLOCK / LANES groups take rows in turn, the next
+// row's loads in flight while this one is worked on.
+template <typename T, typename P, int BLOCK, int LANES, int VPL, int N>
+__global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LayerNormFwd a) {
+  constexpr int ROWS = BLOCK / LANES;
+  static_assert(LANES <= 64 || ROWS == 1, "a barrier belongs to one row");
   __shared__ float lds[2][32];
-  const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  const int lane = threadIdx.x % LANES;
+  const Columns<LANES, VPL, N> at(lane, a.H);
   const float width = (float)a.H;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + grp; row < a.M; row += (int64_t)gridDim.x * ROWS) {
-    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + row_group<LANES>();
+  Pack<T, N> next[VPL];
+  if (row < a.M) load_packs<T>(static_cast<const T*>(a.x) + row * a.ldx, at, next);
+  float g[VPL][N], b[VPL][N];
+  load_weights<P>(a.gamma, at, 1.f, g);
+  load_weights<P>(a.beta, at, 0.f, b);
+  for (; row < a.M; row += step) {
     float v[VPL][N];
     float s = 0.f, zero = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      load_row<T, N>(x, (i * LANES + lane) * N, a.H, 0.f, v[i]);
+    for (int i = 0; i < VPL; ++i)
 #pragma unroll
-      for (int k = 0; k < N; ++k) s += v[i][k];
-    }
+      for (int k = 0; k < N; ++k) {
+        v[i][k] = to_f(next[i].e[k]);
+        s += at.has(i, k) ? v[i][k] : 0.f;
+      }
+    if (row + step < a.M) load_packs<T>(static_cast<const T*>(a.x) + (row + step) * a.ldx, at, next);
     row_sum2<LANES>(s, zero, lds[0]);
     const float mean = s / width;
     float q = 0.f, rest = 0.f, low = 0.f;
@@ -73,11 +133,11 @@ __global__ __launch_bounds__(block_of<LANES>()) void ln_fwd_kernel(LayerNormFwd 
     for (int i = 0; i < VPL; ++i)
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const bool in = (i * LANES + lane) * N + k < a.H;
-        const float x0 = v[i][k], d = in ? x0 - mean : 0.f;
-        low += in ? (x0 - d) - mean : 0.f;  // what the difference was rounded by
-        q += d * d;
-        rest += d;
+        const float d = v[i][k] - mean;
+        const float e = (v[i][k] - d) - mean;  // what the difference was rounded by
+        low += at.has(i, k) ? e : 0.f;
+        q += at.has(i, k) ? d * d : 0.f;
+        rest += at.has(i, k) ? d : 0.f;
         v[i][k] = d;
       }
     rest += low;
@@ -91,18 +151,10 @@ __global__ __launch_bounds__(block_of<LANES>()) void ln_fwd_kernel(LayerNormFwd 
     T* y = static_cast<T*>(a.y) + row * a.H;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const int c = (i * LANES + lane) * N;
-      float g[N], b[N];
+      Pack<T, N> o;
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        g[k] = 1.f;
-        b[k] = 0.f;
-      }
-      if (a.gamma) load_row<P, N>(static_cast<const P*>(a.gamma), c, a.H, 0.f, g);
-      if (a.beta) load_row<P, N>(static_cast<const P*>(a.beta), c, a.H, 0.f, b);
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[i][k] = (v[i][k] - rest) * rstd * g[k] + b[k];
-      store_row<T, N>(y, c, a.H, v[i]);
+      for (int k = 0; k < N; ++k) o.e[k] = from_f<T>((v[i][k] - rest) * rstd * g[i][k] + b[i][k]);
+      if (at.any(i)) store_pack<T, N>(y + at.c[i], o);
     }
   }
 }
@@ -143,42 +195,56 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LayerNormFwd a) {
   }
 }
 
-template <typename T, typename P, int LANES, int VPL>
-__global__ __launch_bounds__(block_of<LANES>()) void ln_bwd_kernel(LayerNormBwd a) {
-  constexpr int N = Vec<T>::N, ROWS = block_of<LANES>() / LANES;
+template <typename T, typename P, int BLOCK, int LANES, int VPL, int N>
+__global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
+  constexpr int ROWS = BLOCK / LANES;
   constexpr int WIDE = LANES * VPL * N;  // columns the registers of a row's lanes hold
+  static_assert(LANES <= 64 || ROWS == 1, "a barrier belongs to one row");
   __shared__ float lds[2][32];
-  __shared__ float sums[ROWS > 1 ? ROWS * WIDE : 1];
-  const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  __shared__ float sums[ROWS > 1 ? ROWS / 2 * WIDE : 1];
+  const int lane = threadIdx.x % LANES, grp = row_group<LANES>();
+  const Columns<LANES, VPL, N> at(lane, a.H);
   const float inv = 1.f / (float)a.H;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + grp;
+  Pack<T, N> nx[VPL], nd[VPL];
+  float mean = 0.f, rstd = 0.f;
+  if (row < a.M) {
+    load_packs<T>(static_cast<const T*>(a.x) + row * a.ldx, at, nx);
+    load_packs<T>(static_cast<const T*>(a.dy) + row * a.lddy, at, nd);
+    mean = a.mean[row];
+    rstd = a.rstd[row];
+  }
   float g[VPL][N], dg[VPL][N], db[VPL][N];
+  load_weights<P>(a.gamma, at, 1.f, g);
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
+  for (int i = 0; i < VPL; ++i)
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      g[i][k] = 1.f;
       dg[i][k] = db[i][k] = 0.f;
+      if (!at.has(i, k)) g[i][k] = 0.f;  // another lane's element adds nothing to the row's sums
     }
-    if (a.gamma) load_row<P, N>(static_cast<const P*>(a.gamma), (i * LANES + lane) * N, a.H, 0.f, g[i]);
-  }
-  int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + grp; row < a.M; row += (int64_t)gridDim.x * ROWS, turn ^= 1) {
-    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
-    const float mean = a.mean[row], rstd = a.rstd[row];
+  for (int turn = 0; row < a.M; row += step, turn ^= 1) {
     float xh[VPL][N], u[VPL][N];
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int c = (i * LANES + lane) * N;
-      load_row<T, N>(x, c, a.H, mean, xh[i]);
-      load_row<T, N>(dy, c, a.H, 0.f, u[i]);
-    }
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        xh[i][k] = (xh[i][k] - mean) * rstd;
+        xh[i][k] = (to_f(nx[i].e[k]) - mean) * rstd;
+        u[i][k] = to_f(nd[i].e[k]);
+      }
+    const float scale = rstd;
+    if (row + step < a.M) {
+      load_packs<T>(static_cast<const T*>(a.x) + (row + step) * a.ldx, at, nx);
+      load_packs<T>(static_cast<const T*>(a.dy) + (row + step) * a.lddy, at, nd);
+      mean = a.mean[row + step];
+      rstd = a.rstd[row + step];
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
         dg[i][k] += u[i][k] * xh[i][k];
         db[i][k] += u[i][k];
         u[i][k] *= g[i][k];
@@ -191,31 +257,49 @@ __global__ __launch_bounds__(block_of<LANES>()) void ln_bwd_kernel(LayerNormBwd 
     T* dx = static_cast<T*>(a.dx) + row * a.H;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
+      Pack<T, N> o;
 #pragma unroll
-      for (int k = 0; k < N; ++k) u[i][k] = rstd * (u[i][k] - s1 - xh[i][k] * s2);
-      store_row<T, N>(dx, (i * LANES + lane) * N, a.H, u[i]);
+      for (int k = 0; k < N; ++k) o.e[k] = from_f<T>(scale * (u[i][k] - s1 - xh[i][k] * s2));
+      if (at.full(i)) {
+        store_pack<T, N>(dx + at.c[i], o);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (at.has(i, k)) dx[at.c[i] + k] = o.e[k];
+      }
     }
   }
   if (!a.part) return;
-  // one row of partial sums for the workgroup: dgamma, then dbeta
+  // one row of partial sums for the workgroup: dgamma, then dbeta; the groups
+  // halve until one is left
   for (int which = 0; which < 2; ++which) {
-    float* out = a.part + ((int64_t)blockIdx.x * 2 + which) * a.H;
-    if constexpr (ROWS == 1) {
+    float(&mine)[VPL][N] = which ? db : dg;
+    if constexpr (ROWS > 1) {
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) store_row<float, N>(out, (i * LANES + lane) * N, a.H, which ? db[i] : dg[i]);
-    } else {
-      __syncthreads();
+      for (int half = ROWS / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (grp >= half && grp < 2 * half) {
+#pragma unroll
+          for (int i = 0; i < VPL; ++i)
+#pragma unroll
+            for (int k = 0; k < N; ++k) sums[(grp - half) * WIDE + (k * VPL + i) * LANES + lane] = mine[i][k];
+        }
+        __syncthreads();
+        if (grp < half) {
+#pragma unroll
+          for (int i = 0; i < VPL; ++i)
+#pragma unroll
+            for (int k = 0; k < N; ++k) mine[i][k] += sums[grp * WIDE + (k * VPL + i) * LANES + lane];
+        }
+      }
+    }
+    float* out = a.part + ((int64_t)blockIdx.x * 2 + which) * a.H;
+    if (grp == 0) {
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
 #pragma unroll
-        for (int k = 0; k < N; ++k) sums[grp * WIDE + (i * LANES + lane) * N + k] = which ? db[i][k] : dg[i][k];
-      __syncthreads();
-      for (int c = threadIdx.x; c < a.H; c += block_of<LANES>()) {
-        float s = 0.f;
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) s += sums[r * WIDE + c];
-        out[c] = s;
-      }
+        for (int k = 0; k < N; ++k)
+          if (at.has(i, k)) out[at.c[i] + k] = mine[i][k];
     }
   }
 }
@@ -263,7 +347,8 @@ __global__ __launch_bounds__(256) void ln_colsum_long_kernel(LayerNormBwd a) {
 }
 
 // dgamma (blockIdx.y = 0) / dbeta (1): the G rows of partials added in a fixed
-// order, 32 columns (a 128-byte line) and 32 row lanes to a workgroup.
+// order, 32 columns (a 128-byte line) and 32 row lanes to a workgroup, eight
+// loads of a lane in flight.
 template <typename P>
 __global__ __launch_bounds__(1024) void ln_wgrad_kernel(const float* __restrict__ part, P* dgamma, P* dbeta, int G,
                                                         int H) {
@@ -272,7 +357,13 @@ __global__ __launch_bounds__(1024) void ln_wgrad_kernel(const float* __restrict_
   const int c = blockIdx.x * 32 + col, which = blockIdx.y;
   float s = 0.f;
   if (c < H)
-    for (int i = r; i < G; i += 32) s += part[((int64_t)i * 2 + which) * H + c];
+    for (int i = r; i < G; i += 8 * 32) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = part[((int64_t)min(i + 32 * j, G - 1) * 2 + which) * H + c];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += i + 32 * j < G ? v[j] : 0.f;
+    }
   lds[r][col] = s;
   __syncthreads();
   if (r == 0 && c < H) {
@@ -284,50 +375,68 @@ __global__ __launch_bounds__(1024) void ln_wgrad_kernel(const float* __restrict_
   }
 }
 
-// Lanes and packs a row takes: the fewest that hold it, so that one load of
-// each lane covers the row as far as possible.  0 lanes: no variant holds it.
-struct Shape {
-  int lanes, vpl;
-};
-Shape shape_of(int H, int type, bool back) {
-  const int n = type == ELEM_F32 ? 4 : 8;
-  const Shape all[] = {{16, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}};
-  for (const Shape& s : all)
-    if (H <= s.lanes * s.vpl * n) return s;
-  return {0, 0};
+// Threads of a workgroup, lanes and packs of a row, elements of a pack: the
+// fewest lanes that hold the row in 16 elements each (with the weights and
+// their sums a backward thread then stays within 128 registers).  Rows of
+// fewer elements than a pack take one element a lane.
+template <typename T, bool BACK, typename F>
+bool with_shape(int H, F&& f) {
+  constexpr int N = Vec<T>::N;
+#define MFL_LN(L_, V_, N_) \
+  if (H <= L_ * V_ * N_) return f(std::integral_constant<int, L_>(), std::integral_constant<int, V_>(), \
+                                  std::integral_constant<int, N_>()), true;
+  if (H < N) {
+    MFL_LN(16, 1, 1)
+  }
+  MFL_LN(16, 1, N)
+  MFL_LN(64, 1, N) MFL_LN(64, 2, N)
+  if constexpr (N == 4 && !BACK) {  // (backward: 32 registers of loads ahead are too many)
+    MFL_LN(64, 4, N)
+  }
+  MFL_LN(256, 1, N) MFL_LN(256, 2, N)
+  if constexpr (N == 4) {
+    MFL_LN(256, 4, N)
+  }
+  MFL_LN(1024, 1, N) MFL_LN(1024, 2, N)
+  if constexpr (N == 4) {
+    MFL_LN(1024, 4, N)
+  }
+#undef MFL_LN
+  return false;
 }
-int rows_of(const Shape& s) { return s.lanes > 256 ? 1 : 256 / s.lanes; }
+constexpr int fwd_block(int lanes) { return lanes > 256 ? lanes : 256; }
+constexpr int bwd_block(int lanes) { return lanes == 256 ? 256 : 1024; }
 
 template <typename T, typename P>
 void fwd_typed(const LayerNormFwd& a, hipStream_t s) {
-  const Shape sh = shape_of(a.H, a.type, false);
-  const int rows = sh.lanes ? rows_of(sh) : 1;
-  const int64_t want = ((int64_t)a.M + rows - 1) / rows;
-  const unsigned grid = (unsigned)(want < (1 << 20) ? want : (1 << 20));
-#define MFL_LN(L_, V_)                                                              \
-  if (sh.lanes == L_ && sh.vpl == V_) {                                             \
-    ln_fwd_kernel<T, P, L_, V_><<<grid, block_of<L_>(), 0, s>>>(a);                 \
-    return;                                                                         \
-  }
-  MFL_LN(16, 1)
-  MFL_LN(64, 1) MFL_LN(64, 2) MFL_LN(64, 4) MFL_LN(256, 2) MFL_LN(256, 4) MFL_LN(1024, 2) MFL_LN(1024, 4)
-#undef MFL_LN
-  ln_fwd_long_kernel<T, P><<<grid, 1024, 0, s>>>(a);
+  const bool done = with_shape<T, false>(a.H, [&](auto L, auto V, auto N) {
+    constexpr int BLOCK = fwd_block(L), ROWS = BLOCK / L;
+    const int64_t want = ((int64_t)a.M + ROWS - 1) / ROWS, cap = 2048 * 256 / BLOCK;
+    ln_fwd_kernel<T, P, BLOCK, L, V, N><<<(unsigned)(want < cap ? want : cap), BLOCK, 0, s>>>(a);
+  });
+  if (!done) ln_fwd_long_kernel<T, P><<<(unsigned)(a.M < (1 << 20) ? a.M : (1 << 20)), 1024, 0, s>>>(a);
+}
+
+// Workgroups of the backward (rows of partial sums): what the chip holds at a
+// time, fewer for few rows.
+template <typename T>
+int bwd_blocks(int M, int H) {
+  int G = M < 64 ? M : 64;
+  with_shape<T, true>(H, [&](auto L, auto, auto) {
+    constexpr int BLOCK = bwd_block(L), ROWS = BLOCK / L;
+    const int want = (int)(((int64_t)M + ROWS - 1) / ROWS), cap = BLOCK == 1024 ? 256 : 512;
+    G = want < cap ? want : cap;
+  });
+  return G;
 }
 
 template <typename T, typename P>
 void bwd_typed(const LayerNormBwd& a, hipStream_t s) {
-  const Shape sh = shape_of(a.H, a.type, true);
-  const int G = layer_norm_bwd_blocks(a.M, a.H, a.type);
-  bool done = false;
-#define MFL_LN(L_, V_)                                                              \
-  if (sh.lanes == L_ && sh.vpl == V_) {                                             \
-    ln_bwd_kernel<T, P, L_, V_><<<G, block_of<L_>(), 0, s>>>(a);                    \
-    done = true;                                                                    \
-  }
-  MFL_LN(16, 1)
-  MFL_LN(64, 1) MFL_LN(64, 2) MFL_LN(64, 4) MFL_LN(256, 2) MFL_LN(256, 4) MFL_LN(1024, 2) MFL_LN(1024, 4)
-#undef MFL_LN
+  const int G = bwd_blocks<T>(a.M, a.H);
+  const bool done = with_shape<T, true>(a.H, [&](auto L, auto V, auto N) {
+    constexpr int BLOCK = bwd_block(L);
+    ln_bwd_kernel<T, P, BLOCK, L, V, N><<<G, BLOCK, 0, s>>>(a);
+  });
   if (!done) {
     ln_bwd_long_kernel<T, P><<<(unsigned)(a.M < (1 << 20) ? a.M : (1 << 20)), 1024, 0, s>>>(a);
     if (a.part) ln_colsum_long_kernel<T><<<dim3((a.H + 255) / 256, G), 256, 0, s>>>(a);
@@ -339,14 +448,8 @@ void bwd_typed(const LayerNormBwd& a, hipStream_t s) {
 
 }  // namespace
 
-// Workgroups of the backward (rows of partial sums): enough to fill the chip
-// four times over, fewer for few rows.
 int layer_norm_bwd_blocks(int M, int H, int type) {
-  const Shape sh = shape_of(H, type, true);
-  if (!sh.lanes) return M < 64 ? M : 64;
-  const int rows = rows_of(sh);
-  const int64_t want = ((int64_t)M + rows - 1) / rows;
-  return (int)(want < 1024 ? want : 1024);
+  return type == ELEM_F32 ? bwd_blocks<float>(M, H) : bwd_blocks<BF16>(M, H);
 }
 
 // Parameters are fp32 or of the input's own type.

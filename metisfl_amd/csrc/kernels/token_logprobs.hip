@@ -331,8 +331,9 @@ template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void logprobs_kernel(TokenLogprobs a) {
   constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
   __shared__ RowShared<THREADS> shared[ROWS];
-  RowShared<THREADS>& sh = shared[threadIdx.x / THREADS];
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS; row < a.N; row += (int64_t)gridDim.x * ROWS) {
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
+  RowShared<THREADS>& sh = shared[group];
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + group; row < a.N; row += (int64_t)gridDim.x * ROWS) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const int64_t t = target_of(a.target64, a.target32, row);
     const bool has = t >= 0 && t < a.V;
