@@ -76,7 +76,7 @@ void launch_token_logprobs_bwd(const TokenLogprobsBwd& a, hipStream_t s);
 
 // ---- AdamW over many tensors ---------------------------------------------------------
 constexpr int kAdamBlock = 128;    // elements that share a scale of the 8-bit states
-constexpr int kAdamChunk = 4096;   // elements of a workgroup
+constexpr int kAdamChunk = 2048;   // elements of a workgroup: 8 to each of 256 threads
 constexpr int kAdamGrads = 384;    // gradient pointers of a launch (kernel arguments hold 4 KB)
 struct AdamTensor {                // one parameter, as the device table holds it
   void* p;

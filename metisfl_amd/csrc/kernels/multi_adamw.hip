@@ -5,7 +5,7 @@
 //
 // Bound by memory: p, m, v are read and written and g read once (28 bytes an
 // element with fp32 states and gradients, 16 with 8-bit states).  The
-// parameters' table and the list of 4096-element chunks live on the device
+// parameters' table and the list of their chunks live on the device
 // from the optimizer's construction; a step hands over only the gradients'
 // addresses, as kernel arguments, so a step is two launches for up to 384
 // tensors and holds in a captured graph.  The first launch (one thread)
@@ -58,7 +58,7 @@ __global__ void adam_begin_kernel(AdamStep a) {
   a.scalars[0] = s;
 }
 
-// 8 states of a thread; 16 threads (a row of the wave) share a scale.
+// 8 codes of a thread as values.
 __device__ __forceinline__ void unpack_states(uint2 w, float scale, float* f) {
   typedef float v2 __attribute__((ext_vector_type(2)));
   const uint32_t u[2] = {w.x, w.y};
@@ -73,155 +73,203 @@ __device__ __forceinline__ void unpack_states(uint2 w, float scale, float* f) {
   }
 }
 
-// Codes of 8 values and the block's 2^E; SHIFT picks the dither's half of the
-// mixed bits, LEAST keeps values above zero above zero.
+// Codes of 8 values and their block's 2^E (16 threads, a row of the wave, have
+// a block).  The conversion with a dither adds the dither's high bits to those
+// a code drops, below 2^-6 too, where codes are 2^-9 apart; HIGH picks the half
+// of the mixed bits, LEAST keeps values above zero above zero.  Infinities
+// become NaN and do not raise the scale.
 template <bool HIGH, bool LEAST>
 __device__ __forceinline__ uint2 pack_states(const float* x, const uint32_t* bits, float* scale) {
-  uint32_t top = 0;
+  float top = 0.f;  // (the maximum passes over NaN)
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t b = __float_as_uint(x[k]) & 0x7fffffffu;
-    if (b < 0x7f800000u && b > top) top = b;
-  }
+  for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
+  top = max16(top);
+  if (top == INFINITY) {
+    top = 0.f;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    const uint32_t w = __shfl_xor(top, o, 64);
-    top = w > top ? w : top;
+    for (int k = 0; k < 8; ++k) top = fabsf(x[k]) < INFINITY ? fmaxf(top, fabsf(x[k])) : top;
+    top = max16(top);
   }
   // biased exponent of 2^E: a block whose largest is below 2^-110 (or zero) takes the least
-  int e = (int)(top >> 23) - 7;
+  int e = (int)(__float_as_uint(top) >> 23) - 7;
   e = e < 10 ? 10 : e;
   *scale = __uint_as_float((uint32_t)e << 23);
   const float up = __uint_as_float((uint32_t)(254 - e) << 23);
-  uint32_t out[2];
+  int out[2] = {0, 0};
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float q[4];
+  for (int k = 0; k < 8; ++k) {
+    float y = x[k] * up;
+    if (LEAST) y = y > 0.f ? fmaxf(y, 0.001953125f) : y;
+    const uint32_t d = HIGH ? bits[k] & 0xffff0000u : bits[k] << 16;
+    int& w = out[k / 4];
+    w = k % 4 == 0   ? __builtin_amdgcn_cvt_sr_fp8_f32(y, d, w, 0)
+        : k % 4 == 1 ? __builtin_amdgcn_cvt_sr_fp8_f32(y, d, w, 1)
+        : k % 4 == 2 ? __builtin_amdgcn_cvt_sr_fp8_f32(y, d, w, 2)
+                     : __builtin_amdgcn_cvt_sr_fp8_f32(y, d, w, 3);
+  }
+  return make_uint2((uint32_t)out[0], (uint32_t)out[1]);
+}
+
+// n (at most 8) elements of any alignment; the others 0
+template <typename T>
+__device__ __forceinline__ Pack<T, 8> load8(const T* p, int n) {
+  if (n >= 8) return load_pack<T, 8>(p);
+  Pack<T, 8> v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int k = 4 * h + i;
-      const float y = fabsf(x[k]) * up;
-      const float low = y < 0.015625f ? 0.015625f : 0.f;  // below 2^-6 the codes are 2^-9 apart
-      const uint32_t d = HIGH ? bits[k] >> 16 : bits[k] & 0xffffu;
-      float z = __uint_as_float((__float_as_uint(y + low) + (d << 4)) & ~0xfffffu) - low;
-      if (LEAST && y > 0.f) z = fmaxf(z, 0.001953125f);
-      z = y < 512.f ? z : __uint_as_float(0x7fc00000u);
-      q[i] = copysignf(z, x[k]);
+  for (int k = 0; k < 8; ++k) v.e[k] = k < n ? p[k] : T{};
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, const Pack<T, 8>& v) {
+  if (n >= 8) {
+    store_pack<T, 8>(p, v);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k < n) p[k] = v.e[k];
+}
+
+// What a thread reads of 8 elements.
+template <int BITS, typename PT, typename GT>
+struct AdamIn {
+  Pack<PT, 8> p;
+  Pack<GT, 8> g;
+  Pack<float, 8> m, v;  // 32 bits
+  uint2 mq, vq;         // 8 bits
+  float ms, vs;
+  __device__ __forceinline__ void load(const PT* pp, const GT* gp, const void* mp, const void* vp, const float* msp,
+                                       const float* vsp, int i, int left) {
+    if constexpr (BITS == 8) {
+      mq = static_cast<const uint2*>(mp)[i >> 3];
+      vq = static_cast<const uint2*>(vp)[i >> 3];
+      ms = msp[i >> 7];
+      vs = vsp[i >> 7];
+    } else {
+      m = load_pack<float, 8>(static_cast<const float*>(mp) + i);
+      v = load_pack<float, 8>(static_cast<const float*>(vp) + i);
     }
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
-    out[h] = (uint32_t)w;
+    p = load8(pp + i, left);
+    g = load8(gp + i, left);
   }
-  return make_uint2(out[0], out[1]);
-}
+};
 
-// 8 elements from i of n (fill 0) and back, any alignment of the tensor
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t i, int64_t n, float* f) {
-  if (i + 8 <= n) {
-    const Pack<T, 8> v = load_pack<T, 8>(p + i);
+// One chunk: elements chunk * kAdamChunk .. of tensor t, 8 to a thread, all of
+// a thread's loads in flight together.  The pointers are the workgroup's (scalars).
+template <int BITS, typename PT, typename GT>
+__device__ __forceinline__ void adam_chunk(const AdamStep& a, const AdamTensor& t, const AdamScalars& sc, const GT* g,
+                                           int chunk) {
+  const int64_t first = (int64_t)chunk * kAdamChunk, at0 = t.offset + first;
+  const int n = (int)(t.numel - first < kAdamChunk ? t.numel - first : kAdamChunk);
+  const int i = threadIdx.x * 8, left = n - i;
+  // whole blocks of 128: the 16 threads of a scale stay together
+  if (i >= ((n + kAdamBlock - 1) & ~(kAdamBlock - 1))) return;
+  PT* p0 = static_cast<PT*>(t.p) + first;
+  BF16* mirror = t.mirror ? reinterpret_cast<BF16*>(t.mirror) + first : nullptr;
+  const int state = BITS == 8 ? 1 : 4;
+  char* m0 = static_cast<char*>(a.m) + at0 * state;
+  char* v0 = static_cast<char*>(a.v) + at0 * state;
+  float* ms0 = BITS == 8 ? a.m_scale + at0 / kAdamBlock : nullptr;
+  float* vs0 = BITS == 8 ? a.v_scale + at0 / kAdamBlock : nullptr;
+  const float b1 = (float)a.beta1, b2 = (float)a.beta2, n1 = (float)(1.0 - a.beta1), n2 = (float)(1.0 - a.beta2);
+  AdamIn<BITS, PT, GT> in;
+  in.load(p0, g + first, m0, v0, ms0, vs0, i, left);
+  float p[8], m[8], v[8], r[8];
+  uint32_t bits[8];
+  if constexpr (BITS == 8) {
+    unpack_states(in.mq, in.ms, m);
+    unpack_states(in.vq, in.vs, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = to_f(v.e[k]);
+    for (int k = 0; k < 8; ++k) v[k] = v[k] * v[k];
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = i + k < n ? to_f(p[i + k]) : 0.f;
+    for (int k = 0; k < 8; ++k) {
+      m[k] = in.m.e[k];
+      v[k] = in.v.e[k];
+    }
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int64_t i, int64_t n, const T* v) {
-  if (i + 8 <= n) {
-    __builtin_memcpy(p + i, v, 8 * sizeof(T));
-  } else {
+  const int64_t at = at0 + i;
+  const uint32_t high = (uint32_t)(at >> 32) * 0x9E3779B1u;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i + k < n) p[i + k] = v[k];
+  for (int k = 0; k < 8; ++k) {
+    const float gk = to_f(in.g.e[k]), pk = to_f(in.p.e[k]);
+    m[k] = m[k] * b1 + gk * n1;
+    v[k] = v[k] * b2 + (gk * n2) * gk;
+    r[k] = sqrtf(v[k]);
+    p[k] = pk - ((m[k] * sc.c1) / (r[k] * sc.c2 + a.eps) + pk * t.wd) * sc.lr;
+    if (BITS == 8 || sizeof(PT) == 2) bits[k] = mix32((((uint32_t)at + k) ^ sc.key) + high);
+  }
+  if constexpr (BITS == 8) {
+    float ms, vs;
+    const uint2 mq = pack_states<false, false>(m, bits, &ms);
+    const uint2 vq = pack_states<true, true>(r, bits, &vs);
+    reinterpret_cast<uint2*>(m0)[i >> 3] = mq;
+    reinterpret_cast<uint2*>(v0)[i >> 3] = vq;
+    if ((threadIdx.x & 15) == 0) {
+      ms0[i >> 7] = ms;
+      vs0[i >> 7] = vs;
+    }
+  } else {
+    Pack<float, 8> mo, vo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      mo.e[k] = m[k];
+      vo.e[k] = v[k];
+    }
+    store_pack<float, 8>(reinterpret_cast<float*>(m0) + i, mo);
+    store_pack<float, 8>(reinterpret_cast<float*>(v0) + i, vo);
+  }
+  Pack<PT, 8> po;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (sizeof(PT) == 2) {
+      const uint32_t b = __float_as_uint(p[k]);
+      if (fabsf(p[k]) < INFINITY) p[k] = __uint_as_float((b + (mix32(bits[k]) >> 16)) & 0xffff0000u);
+    }
+    po.e[k] = from_f<PT>(p[k]);
+  }
+  store8(p0 + i, left, po);
+  if (mirror) {
+    Pack<BF16, 8> q;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q.e[k] = from_f<BF16>(p[k]);
+    store8(mirror + i, left, q);
   }
 }
 
-__device__ __forceinline__ void load_grad(const void* g, int type, int64_t i, int64_t n, float* f) {
-  if (type == ELEM_F32) load8(static_cast<const float*>(g), i, n, f);
-  else if (type == ELEM_BF16) load8(static_cast<const BF16*>(g), i, n, f);
-  else load8(static_cast<const F16*>(g), i, n, f);
+// Read-only tables through scalar loads.
+template <typename T>
+__device__ __forceinline__ T table_entry(const T* table, int64_t i) {
+  typedef const __attribute__((address_space(4))) uint32_t* Words;
+  const Words w = (Words)(uintptr_t)(table + i);
+  uint32_t words[sizeof(T) / 4];
+#pragma unroll
+  for (size_t k = 0; k < sizeof(T) / 4; ++k) words[k] = w[k];
+  T v;
+  __builtin_memcpy(&v, words, sizeof(T));
+  return v;
 }
 
 template <int BITS>
 __global__ __launch_bounds__(256) void adam_chunk_kernel(AdamStep a, AdamGrads grads, int first_tensor,
                                                          int64_t first_chunk) {
-  const AdamChunk ch = a.chunks[first_chunk + blockIdx.x];
+  const AdamChunk ch = table_entry(a.chunks, first_chunk + blockIdx.x);
   const void* g = grads.g[ch.tensor - first_tensor];
   if (!g) return;  // no gradient: the tensor and its states stay as they are
   const int gtype = grads.type[ch.tensor - first_tensor];
-  const AdamTensor t = a.tensors[ch.tensor];
-  const AdamScalars sc = a.scalars[0];
-  const float b1 = (float)a.beta1, b2 = (float)a.beta2, n1 = (float)(1.0 - a.beta1), n2 = (float)(1.0 - a.beta2);
-  const int64_t end = t.numel < (int64_t)(ch.chunk + 1) * kAdamChunk ? t.numel : (int64_t)(ch.chunk + 1) * kAdamChunk;
-  // whole blocks of 128: the 16 threads of a scale stay together
-  for (int64_t i = (int64_t)ch.chunk * kAdamChunk + threadIdx.x * 8; i < ((end + kAdamBlock - 1) & ~(int64_t)(kAdamBlock - 1));
-       i += 2048) {
-    float gf[8], p[8], m[8], v[8], r[8];
-    load_grad(g, gtype, i, end, gf);
-    if (t.param_type == ELEM_F32) load8(static_cast<const float*>(t.p), i, end, p);
-    else load8(static_cast<const BF16*>(t.p), i, end, p);
-    const int64_t at = t.offset + i;
-    if constexpr (BITS == 8) {
-      unpack_states(reinterpret_cast<const uint2*>(a.m)[at >> 3], a.m_scale[at >> 7], m);
-      unpack_states(reinterpret_cast<const uint2*>(a.v)[at >> 3], a.v_scale[at >> 7], v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = v[k] * v[k];
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        *reinterpret_cast<float4*>(m + 4 * h) = reinterpret_cast<const float4*>(a.m)[(at >> 2) + h];
-        *reinterpret_cast<float4*>(v + 4 * h) = reinterpret_cast<const float4*>(a.v)[(at >> 2) + h];
-      }
-    }
-    uint32_t bits[8];
-    const uint32_t high = (uint32_t)(at >> 32) * 0x9E3779B1u;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      m[k] = m[k] * b1 + gf[k] * n1;
-      v[k] = v[k] * b2 + (gf[k] * n2) * gf[k];
-      r[k] = sqrtf(v[k]);
-      p[k] = p[k] - ((m[k] * sc.c1) / (r[k] * sc.c2 + a.eps) + p[k] * t.wd) * sc.lr;
-      bits[k] = mix32((((uint32_t)at + k) ^ sc.key) + high);
-    }
-    if constexpr (BITS == 8) {
-      float ms, vs;
-      const uint2 mq = pack_states<false, false>(m, bits, &ms);
-      const uint2 vq = pack_states<true, true>(r, bits, &vs);
-      reinterpret_cast<uint2*>(a.m)[at >> 3] = mq;
-      reinterpret_cast<uint2*>(a.v)[at >> 3] = vq;
-      if ((threadIdx.x & 15) == 0) {
-        a.m_scale[at >> 7] = ms;
-        a.v_scale[at >> 7] = vs;
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        reinterpret_cast<float4*>(a.m)[(at >> 2) + h] = *reinterpret_cast<float4*>(m + 4 * h);
-        reinterpret_cast<float4*>(a.v)[(at >> 2) + h] = *reinterpret_cast<float4*>(v + 4 * h);
-      }
-    }
-    if (t.param_type == ELEM_F32) {
-      store8(static_cast<float*>(t.p), i, end, p);
-    } else {
-      BF16 q[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t b = __float_as_uint(p[k]);
-        const bool finite = (b & 0x7f800000u) != 0x7f800000u;
-        if (finite) p[k] = __uint_as_float((b + (mix32(bits[k]) >> 16)) & 0xffff0000u);
-        q[k] = from_f<BF16>(p[k]);
-      }
-      store8(static_cast<BF16*>(t.p), i, end, q);
-    }
-    if (t.mirror) {
-      BF16 q[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) q[k] = from_f<BF16>(p[k]);
-      store8(reinterpret_cast<BF16*>(t.mirror), i, end, q);
-    }
+  const AdamTensor t = table_entry(a.tensors, ch.tensor);
+  const AdamScalars sc = table_entry(a.scalars, 0);
+#define MFL_ADAM(P_, G_) adam_chunk<BITS, P_, G_>(a, t, sc, static_cast<const G_*>(g), ch.chunk)
+  if (t.param_type == ELEM_F32) {
+    if (gtype == ELEM_F32) MFL_ADAM(float, float);
+    else if (gtype == ELEM_BF16) MFL_ADAM(float, BF16);
+    else MFL_ADAM(float, F16);
+  } else {
+    if (gtype == ELEM_F32) MFL_ADAM(BF16, float);
+    else if (gtype == ELEM_BF16) MFL_ADAM(BF16, BF16);
+    else MFL_ADAM(BF16, F16);
   }
+#undef MFL_ADAM
 }
 
 }  // namespace
