@@ -73,6 +73,10 @@ __device__ __forceinline__ float max16(float v) {
   v = fmaxf(v, row_ror<2>(v));
   return fmaxf(v, row_ror<1>(v));
 }
+__device__ __forceinline__ float max4(float v) {  // of a quad
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, false)));  // 1 0 3 2
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4e, 0xf, 0xf, false)));  // 2 3 0 1
+}
 // Sum over aligned groups of L (16 or 64) lanes.
 template <int L>
 __device__ __forceinline__ float lane_sum(float v) {

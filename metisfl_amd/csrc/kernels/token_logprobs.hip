@@ -27,7 +27,7 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kList = 1024;  // candidates of a row (LDS)
-constexpr int kSplitRows = 128, kSplitWidth = 32768, kSplitGroups = 512;  // see part_span
+constexpr int kSplitRows = 128, kSplitWidth = 98304, kSplitGroups = 512;  // see part_span
 
 // Running maximum m, sum of exp(x - m) and sum of exp(x - m) (x - m) log2 e.
 // exp(x - m) = exp2(x L - fl(m L)) with L = log2 e is one fused multiply-add
@@ -106,7 +106,8 @@ template <int THREADS>
 struct RowShared {
   float m[16], s[16], t[16];
   float group[64];
-  int bound, count;
+  float bound;
+  int count;
   uint64_t best[16], top[kTopMax], list[THREADS > 64 ? kList : 256];
 };
 
@@ -116,11 +117,11 @@ __device__ __forceinline__ void row_sync() {
   else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"), __builtin_amdgcn_wave_barrier();
 }
 
-// What a thread saw of the row: its largest element, the batch (packs b * THREADS
-// + tid, ... of its loop) that had it, and the largest of its other batches.
+// What a thread saw of the row: the largest element of each of its two batches
+// with the largest ones, those batches, and the largest element of the others.
 struct Seen {
-  float largest, others;
-  int batch;
+  float largest, second, others;
+  int batch, batch2;
 };
 constexpr int kUnroll = 4;  // packs of a batch: the loads in flight of a thread
 
@@ -163,9 +164,10 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, Seen seen, Row
   float g = seen.largest;
   if constexpr (GROUP == 16) {
     g = max16(g);
-  } else if constexpr (GROUP == 4) {
-    g = fmaxf(g, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(g), 0xb1, 0xf, 0xf, false)));  // 1 0 3 2
-    g = fmaxf(g, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(g), 0x4e, 0xf, 0xf, false)));  // 2 3 0 1
+  } else if constexpr (GROUP > 1) {
+    g = max4(g);
+    if constexpr (GROUP == 8)  // the eight lanes mirrored
+      g = fmaxf(g, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(g), 0x141, 0xf, 0xf, false)));
   }
   if constexpr (GROUP > 1) {
     if (tid % GROUP == 0) sh.group[tid / GROUP] = g;
@@ -174,44 +176,52 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, Seen seen, Row
   }
   if (tid < 64) {  // (the first wave)
     int above = 0;  // groups above this lane's
+    if (K <= 8) {   // four groups together: 16 to rank, about K log 2 elements more above the bound
+      g = max4(g);
 #pragma unroll
-    for (int j = 0; j < 64; ++j) above += lane_of(g, j) > g;
+      for (int j = 0; j < 64; j += 4) above += lane_of(g, j) > g;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) above += lane_of(g, j) > g;
+    }
     const float least = -max64(above < K ? -g : -INFINITY);
     if (tid == 0) {
-      sh.bound = order_of(least);
+      sh.bound = least;
       sh.count = 0;
     }
   }
   row_sync<THREADS>();
-  const int bound = sh.bound;
-  // threads that saw an element of that size list theirs
+  const float bound = sh.bound;
+  // threads that saw an element of that size list theirs (and NaN, which ranks
+  // lowest: it is never below the bound)
   const int packs = n / N, batches = (packs + THREADS * kUnroll - 1) / (THREADS * kUnroll);
-  if (packs && order_of(seen.largest) >= bound) {
-    const bool one = seen.batch >= 0 && order_of(seen.others) < bound;
-    for (int b = one ? seen.batch : 0; b < (one ? seen.batch + 1 : batches); ++b) {
+  auto list = [&](int id) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < CAP) sh.list[at] = rank_key(order_of(to_f(x[id])), first + (uint32_t)id);
+  };
+  if (packs && !(seen.largest < bound)) {
+    const bool few = seen.batch >= 0 && seen.others < bound;
+    const int turns = !few ? batches : seen.second < bound ? 1 : 2;
+    for (int turn = 0; turn < turns; ++turn) {
+      const int b = !few ? turn : turn ? seen.batch2 : seen.batch;
       Batch<T, THREADS> v;
       v.load(x, b, packs);
+      uint32_t mask = 0;  // a bit an element: their values are read again (from L1)
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const int i = (b * kUnroll + u) * THREADS + tid;
+        const bool in = (b * kUnroll + u) * THREADS + tid < packs;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const int o = order_of(to_f(v.v[u].e[k]));
-          if (i < packs && o >= bound) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < CAP) sh.list[at] = rank_key(o, first + (uint32_t)(i * N + k));
-          }
-        }
+        for (int k = 0; k < N; ++k)
+          mask |= in && !(to_f(v.v[u].e[k]) < bound) ? 1u << (u * N + k) : 0u;
+      }
+      for (; mask; mask &= mask - 1) {
+        const int e = __ffs(mask) - 1;
+        list(((b * kUnroll + e / N) * THREADS + tid) * N + e % N);
       }
     }
   }
-  if (packs * N + tid < n) {  // behind the last whole pack: one element of the first threads
-    const int o = order_of(to_f(x[packs * N + tid]));
-    if (o >= bound) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < CAP) sh.list[at] = rank_key(o, first + (uint32_t)(packs * N + tid));
-    }
-  }
+  // behind the last whole pack: one element of the first threads
+  if (packs * N + tid < n && !(to_f(x[packs * N + tid]) < bound)) list(packs * N + tid);
   row_sync<THREADS>();
   const int count = sh.count;
   if (count <= CAP) {
@@ -249,32 +259,32 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, Seen seen, Row
 }
 
 // One pass over x[0 .. n): the row's sums in all its threads, and what this
-// thread saw.
+// thread saw.  `v` holds batch 0 and comes back with that of `then` (null: with
+// nothing), in flight while the row is finished.
 template <typename T, int THREADS>
-__device__ __forceinline__ Soft row_pass(const T* x, int n, Seen& seen, RowShared<THREADS>& sh) {
+__device__ __forceinline__ Soft row_pass(const T* x, int n, const T* then, Batch<T, THREADS>& v, Seen& seen,
+                                         RowShared<THREADS>& sh) {
   constexpr int N = Vec<T>::N;
   const int tid = threadIdx.x % THREADS;
   const int packs = n / N, batches = (packs + THREADS * kUnroll - 1) / (THREADS * kUnroll);
   Soft a = {-INFINITY, 0.f, 0.f};
-  seen = {-INFINITY, -INFINITY, -1};
+  seen = {-INFINITY, -INFINITY, -INFINITY, -1, -1};
   float tail = -INFINITY;
   if (packs * N + tid < n) tail = to_f(x[packs * N + tid]);
-  Batch<T, THREADS> v;
-  if (batches) v.load(x, 0, packs);
   for (int b = 0; b < batches; ++b) {
     float f[kUnroll * N];
     v.get(b, packs, f);
-    if (b + 1 < batches) v.load(x, b + 1, packs);  // in flight while this batch is added
+    const bool more = b + 1 < batches;  // in flight while this batch is added
+    if (more || then) v.load(more ? x : then, more ? b + 1 : 0, packs);
     float largest = f[0];
 #pragma unroll
     for (int k = 1; k < kUnroll * N; ++k) largest = fmaxf(largest, f[k]);
-    if (largest > seen.largest) {
-      seen.others = seen.largest;
-      seen.largest = largest;
-      seen.batch = b;
-    } else {
-      seen.others = fmaxf(seen.others, largest);
-    }
+    const bool first = largest > seen.largest, next = largest > seen.second;
+    seen.others = fmaxf(seen.others, next ? seen.second : largest);
+    seen.second = first ? seen.largest : next ? largest : seen.second;
+    seen.batch2 = first ? seen.batch : next ? b : seen.batch2;
+    seen.largest = first ? largest : seen.largest;
+    seen.batch = first ? b : seen.batch;
     soft_add<kUnroll * N>(a, f, largest);
   }
   soft_add<1>(a, &tail, tail);
@@ -333,13 +343,18 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void logprobs_kernel
   __shared__ RowShared<THREADS> shared[ROWS];
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
   RowShared<THREADS>& sh = shared[group];
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + group; row < a.N; row += (int64_t)gridDim.x * ROWS) {
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + group;
+  const int packs = a.V / Vec<T>::N;
+  Batch<T, THREADS> v;
+  if (row < a.N && packs) v.load(static_cast<const T*>(a.x) + row * a.ldx, 0, packs);
+  for (; row < a.N; row += step) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const int64_t t = target_of(a.target64, a.target32, row);
     const bool has = t >= 0 && t < a.V;
     const float given = has ? to_f(x[t]) : 0.f;  // the target's logit, on its way during the pass
     Seen seen;
-    const Soft r = row_pass<T, THREADS>(x, a.V, seen, sh);
+    const Soft r = row_pass<T, THREADS>(x, a.V, row + step < a.N ? x + step * a.ldx : nullptr, v, seen, sh);
     if (a.K) row_top<T, THREADS>(x, a.V, 0, a.K, seen, sh);
     row_write<T, THREADS>(a, row, r, has, given, sh);
     row_sync<THREADS>();
@@ -359,7 +374,9 @@ __global__ __launch_bounds__(256) void logprobs_part_kernel(TokenLogprobs a, int
   const int lo = part * span, n = min(span, a.V - lo);
   const T* x = static_cast<const T*>(a.x) + row * a.ldx + lo;
   Seen seen;
-  const Soft r = row_pass<T, 256>(x, n, seen, sh);
+  Batch<T, 256> v;
+  if (n >= Vec<T>::N) v.load(x, 0, n / Vec<T>::N);
+  const Soft r = row_pass<T, 256>(x, n, nullptr, v, seen, sh);
   const int K = min(a.K, n);
   if (K) row_top<T, 256>(x, n, (uint32_t)lo, K, seen, sh);
   PartSums* sums = static_cast<PartSums*>(a.work);
@@ -407,8 +424,10 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(TokenLogprobs a, int 
   row_sync<64>();
   row_write<T, 64>(a, row, r, has, given, sh);
 }
-// Elements of a part, or 0 for rows that are not split: only rows that leave
-// most of the chip idle are, into batches of 256 threads, at most 64.
+// Elements of a part, or 0 for rows that are not split: only long rows that
+// leave most of the chip idle are, into batches of 256 threads, at most 64
+// (bf16, 32 rows: 200000 logits 9.9 us against 17.5 us, 65000 10 against 8.5,
+// the join's launch being 2 us).
 int part_span(int N, int V, int type) {
   const int batch = 256 * kUnroll * (type == ELEM_F32 ? 4 : 8);
   if (N > kSplitRows || V < kSplitWidth) return 0;
@@ -498,14 +517,18 @@ void fwd_typed(const TokenLogprobs& a, hipStream_t s) {
     logprobs_join_kernel<T><<<a.N, 64, 0, s>>>(a, parts);
     return;
   }
-  if (a.V <= 2048) {
-    const int64_t want = ((int64_t)a.N + 3) / 4;
-    logprobs_kernel<T, 64><<<(unsigned)(want < cap ? want : cap), 256, 0, s>>>(a);
-  } else if (a.N >= 1024) {
+  // Threads to a row, both sides measured (bf16, 4160 rows, 5 alternatives):
+  // a wave where rows are short, up to 16384 if there are enough to fill the
+  // chip (8000: 25 us against 31 us; 30522: 81 against 64), else 256 up to
+  // 64 KB (30522: 64 against 83 us with 512) and 512 above (128000: 188
+  // against 194; 130 rows: 16 against 20).
+  const int64_t few = (a.N + 3) / 4;
+  if (a.V <= 2048 || (a.V <= 16384 && a.N >= 2048))
+    logprobs_kernel<T, 64><<<(unsigned)(few < cap ? few : cap), 256, 0, s>>>(a);
+  else if ((int64_t)a.V * (int64_t)sizeof(T) <= 65536)
     logprobs_kernel<T, 256><<<(unsigned)(a.N < cap ? a.N : cap), 256, 0, s>>>(a);
-  } else {
-    logprobs_kernel<T, 1024><<<(unsigned)(a.N < cap ? a.N : cap), 1024, 0, s>>>(a);
-  }
+  else
+    logprobs_kernel<T, 512><<<(unsigned)(a.N < cap ? a.N : cap), 512, 0, s>>>(a);
 }
 template <typename T>
 void bwd_typed(const TokenLogprobsBwd& a, hipStream_t s) {
