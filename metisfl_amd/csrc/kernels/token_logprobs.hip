@@ -209,10 +209,10 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, Seen seen, Row
       uint32_t mask = 0;  // a bit an element: their values are read again (from L1)
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const bool in = (b * kUnroll + u) * THREADS + tid < packs;
+        uint32_t part = 0;
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-          mask |= in && !(to_f(v.v[u].e[k]) < bound) ? 1u << (u * N + k) : 0u;
+        for (int k = 0; k < N; ++k) part |= to_f(v.v[u].e[k]) < bound ? 0u : 1u << k;
+        mask |= (b * kUnroll + u) * THREADS + tid < packs ? part << (u * N) : 0u;
       }
       for (; mask; mask &= mask - 1) {
         const int e = __ffs(mask) - 1;
@@ -338,7 +338,7 @@ __device__ __forceinline__ void row_write(const TokenLogprobs& a, int64_t row, S
 }
 
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void logprobs_kernel(TokenLogprobs a) {
+__global__ __launch_bounds__(THREADS > 256 ? THREADS : 256, 5) void logprobs_kernel(TokenLogprobs a) {
   constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
   __shared__ RowShared<THREADS> shared[ROWS];
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
