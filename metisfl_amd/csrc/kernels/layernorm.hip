@@ -7,10 +7,8 @@
 // reads x and dy and writes dx, each once.  LANES lanes hold a row in
 // registers (16 lanes for narrow rows, a wave, 256 or 1024 threads), VPL
 // packs of 16 bytes each, so mean and variance are two passes over registers
-// (no cancellation of E[x^2] - mean^2); the second also sums x - mean and what
-// these differences were rounded by (x of few bits round alike, so it would
-// not average out), which is what the fp32 mean is off by, and corrects it: a
-// constant row gives 0.  The weights' gradients are sums over
+// (no cancellation of E[x^2] - mean^2); the second also sums x - mean, which
+// is what the fp32 mean is off by (row_rest).  The weights' gradients are sums over
 // all rows: each workgroup keeps the partial sums of its columns in registers
 // over its rows, writes one row of partials, and a second launch adds the
 // workgroups' rows in a fixed order, so results repeat bit for bit (no
@@ -64,11 +62,12 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* buf) {
 // column c[i]; one that would end behind the row (or lie there) is moved back
 // to end with it, and its first skip[i] elements, another lane's, count for
 // nothing.  So every load is whole and in the row, whatever its width (>= N).
-template <int LANES, int VPL, int N>
+// EXACT: the row is as wide as the packs, nothing is skipped.
+template <int LANES, int VPL, int N, bool EXACT>
 struct Columns {
   int c[VPL], skip[VPL];
   // shapes hold a row in no more packs than needed: the first ones are whole
-  static constexpr bool whole(int i) { return VPL > 1 && i < VPL / 2; }
+  static constexpr bool whole(int i) { return EXACT || (VPL > 1 && i < VPL / 2); }
   __device__ __forceinline__ Columns(int lane, int H) {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -79,15 +78,14 @@ struct Columns {
   }
   __device__ __forceinline__ bool has(int i, int k) const { return whole(i) || k >= skip[i]; }
   __device__ __forceinline__ bool full(int i) const { return whole(i) || skip[i] == 0; }
-  __device__ __forceinline__ bool any(int i) const { return whole(i) || skip[i] < N; }
 };
-template <typename T, int LANES, int VPL, int N>
-__device__ __forceinline__ void load_packs(const T* row, const Columns<LANES, VPL, N>& at, Pack<T, N> (&v)[VPL]) {
+template <typename T, int LANES, int VPL, int N, bool EXACT>
+__device__ __forceinline__ void load_packs(const T* row, const Columns<LANES, VPL, N, EXACT>& at, Pack<T, N> (&v)[VPL]) {
 #pragma unroll
   for (int i = 0; i < VPL; ++i) v[i] = load_pack<T, N>(row + at.c[i]);
 }
-template <typename P, int LANES, int VPL, int N>
-__device__ __forceinline__ void load_weights(const void* p, const Columns<LANES, VPL, N>& at, float none,
+template <typename P, int LANES, int VPL, int N, bool EXACT>
+__device__ __forceinline__ void load_weights(const void* p, const Columns<LANES, VPL, N, EXACT>& at, float none,
                                              float (&w)[VPL][N]) {
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
@@ -98,15 +96,45 @@ __device__ __forceinline__ void load_weights(const void* p, const Columns<LANES,
   }
 }
 
+template <typename T, int LANES, int VPL, int N, bool EXACT>
+__device__ __forceinline__ void store_packs(T* row, const Columns<LANES, VPL, N, EXACT>& at, const float (&f)[VPL][N]) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    Pack<T, N> o;
+#pragma unroll
+    for (int k = 0; k < N; ++k) o.e[k] = from_f<T>(f[i][k]);
+    if (at.full(i)) {
+      store_pack<T, N>(row + at.c[i], o);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (at.has(i, k)) row[at.c[i] + k] = o.e[k];
+    }
+  }
+}
+
+// 1 / sqrt(variance + eps) from the mean square of x - mean and the mean of
+// x - mean, `rest`, which is what the fp32 mean is off by.
+__device__ __forceinline__ float row_rstd(float square, float rest, float eps) {
+  const float var = square - rest * rest;
+  return 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);
+}
+// The correction of the mean.  Rows far from zero need it, and there x - mean
+// is exact; near zero the differences are rounded, alike for x of few bits, and
+// the sum itself is nearer.
+__device__ __forceinline__ float row_rest(float mean, float rest, float rstd) {
+  return fabsf(mean) * rstd > 1.f ? rest : 0.f;
+}
+
 // A workgroup's rows: its BLOCK / LANES groups take rows in turn, the next
 // row's loads in flight while this one is worked on.
-template <typename T, typename P, int BLOCK, int LANES, int VPL, int N>
+template <typename T, typename P, int BLOCK, int LANES, int VPL, int N, bool EXACT>
 __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LayerNormFwd a) {
   constexpr int ROWS = BLOCK / LANES;
   static_assert(LANES <= 64 || ROWS == 1, "a barrier belongs to one row");
   __shared__ float lds[2][32];
   const int lane = threadIdx.x % LANES;
-  const Columns<LANES, VPL, N> at(lane, a.H);
+  const Columns<LANES, VPL, N, EXACT> at(lane, a.H);
   const float width = (float)a.H;
   const int64_t step = (int64_t)gridDim.x * ROWS;
   int64_t row = (int64_t)blockIdx.x * ROWS + row_group<LANES>();
@@ -122,40 +150,36 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LayerNormFwd a) {
     for (int i = 0; i < VPL; ++i)
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        v[i][k] = to_f(next[i].e[k]);
-        s += at.has(i, k) ? v[i][k] : 0.f;
+        v[i][k] = at.has(i, k) ? to_f(next[i].e[k]) : 0.f;
+        s += v[i][k];
       }
     if (row + step < a.M) load_packs<T>(static_cast<const T*>(a.x) + (row + step) * a.ldx, at, next);
     row_sum2<LANES>(s, zero, lds[0]);
-    const float mean = s / width;
-    float q = 0.f, rest = 0.f, low = 0.f;
+    float mean = s / width;
+    float q = 0.f, rest = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float d = v[i][k] - mean;
-        const float e = (v[i][k] - d) - mean;  // what the difference was rounded by
-        low += at.has(i, k) ? e : 0.f;
-        q += at.has(i, k) ? d * d : 0.f;
-        rest += at.has(i, k) ? d : 0.f;
-        v[i][k] = d;
+        v[i][k] = at.has(i, k) ? v[i][k] - mean : 0.f;
+        q = fmaf(v[i][k], v[i][k], q);
+        rest += v[i][k];
       }
-    rest += low;
     row_sum2<LANES>(q, rest, lds[1]);
     rest /= width;
-    const float var = q / width - rest * rest, rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
+    const float rstd = row_rstd(q / width, rest, a.eps);
+    rest = row_rest(mean, rest, rstd);
+    mean += rest;
     if (lane == 0) {
-      a.mean[row] = mean + rest;
+      a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
-    T* y = static_cast<T*>(a.y) + row * a.H;
+    const float shift = -rest * rstd;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      Pack<T, N> o;
+    for (int i = 0; i < VPL; ++i)
 #pragma unroll
-      for (int k = 0; k < N; ++k) o.e[k] = from_f<T>((v[i][k] - rest) * rstd * g[i][k] + b[i][k]);
-      if (at.any(i)) store_pack<T, N>(y + at.c[i], o);
-    }
+      for (int k = 0; k < N; ++k) v[i][k] = fmaf(fmaf(v[i][k], rstd, shift), g[i][k], b[i][k]);
+    store_packs<T>(static_cast<T*>(a.y) + row * a.H, at, v);
   }
 }
 
@@ -171,17 +195,16 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LayerNormFwd a) {
     for (int c = threadIdx.x; c < a.H; c += 1024) s += to_f(x[c]);
     row_sum2<1024>(s, zero, lds[0]);
     const float mean = s / width;
-    float q = 0.f, rest = 0.f, low = 0.f;
+    float q = 0.f, rest = 0.f;
     for (int c = threadIdx.x; c < a.H; c += 1024) {
-      const float x0 = to_f(x[c]), d = x0 - mean;
-      low += (x0 - d) - mean;
-      q += d * d;
+      const float d = to_f(x[c]) - mean;
+      q = fmaf(d, d, q);
       rest += d;
     }
-    rest += low;
     row_sum2<1024>(q, rest, lds[1]);
     rest /= width;
-    const float var = q / width - rest * rest, rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
+    const float rstd = row_rstd(q / width, rest, a.eps);
+    rest = row_rest(mean, rest, rstd);
     if (threadIdx.x == 0) {
       a.mean[row] = mean + rest;
       a.rstd[row] = rstd;
@@ -195,7 +218,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LayerNormFwd a) {
   }
 }
 
-template <typename T, typename P, int BLOCK, int LANES, int VPL, int N>
+template <typename T, typename P, int BLOCK, int LANES, int VPL, int N, bool EXACT>
 __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
   constexpr int ROWS = BLOCK / LANES;
   constexpr int WIDE = LANES * VPL * N;  // columns the registers of a row's lanes hold
@@ -203,7 +226,7 @@ __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
   __shared__ float lds[2][32];
   __shared__ float sums[ROWS > 1 ? ROWS / 2 * WIDE : 1];
   const int lane = threadIdx.x % LANES, grp = row_group<LANES>();
-  const Columns<LANES, VPL, N> at(lane, a.H);
+  const Columns<LANES, VPL, N, EXACT> at(lane, a.H);
   const float inv = 1.f / (float)a.H;
   const int64_t step = (int64_t)gridDim.x * ROWS;
   int64_t row = (int64_t)blockIdx.x * ROWS + grp;
@@ -254,20 +277,11 @@ __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
     row_sum2<LANES>(s1, s2, lds[turn]);
     s1 *= inv;
     s2 *= inv;
-    T* dx = static_cast<T*>(a.dx) + row * a.H;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      Pack<T, N> o;
+    for (int i = 0; i < VPL; ++i)
 #pragma unroll
-      for (int k = 0; k < N; ++k) o.e[k] = from_f<T>(scale * (u[i][k] - s1 - xh[i][k] * s2));
-      if (at.full(i)) {
-        store_pack<T, N>(dx + at.c[i], o);
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          if (at.has(i, k)) dx[at.c[i] + k] = o.e[k];
-      }
-    }
+      for (int k = 0; k < N; ++k) u[i][k] = scale * (u[i][k] - s1 - xh[i][k] * s2);
+    store_packs<T>(static_cast<T*>(a.dx) + row * a.H, at, u);
   }
   if (!a.part) return;
   // one row of partial sums for the workgroup: dgamma, then dbeta; the groups
@@ -375,27 +389,44 @@ __global__ __launch_bounds__(1024) void ln_wgrad_kernel(const float* __restrict_
   }
 }
 
-// Threads of a workgroup, lanes and packs of a row, elements of a pack: the
-// fewest lanes that hold the row in 16 elements each (with the weights and
-// their sums a backward thread then stays within 128 registers).  Rows of
-// fewer elements than a pack take one element a lane.
+// Lanes and packs of a row, elements of a pack (16 bytes, or 8 where that
+// leaves fewer lanes idle), exactness: the fewest lanes that hold the row in
+// 16 elements each (with the weights and their sums a backward thread then
+// stays within 128 registers).  Rows of fewer elements than a pack take one
+// element a lane.
 template <typename T, bool BACK, typename F>
 bool with_shape(int H, F&& f) {
   constexpr int N = Vec<T>::N;
-#define MFL_LN(L_, V_, N_) \
-  if (H <= L_ * V_ * N_) return f(std::integral_constant<int, L_>(), std::integral_constant<int, V_>(), \
-                                  std::integral_constant<int, N_>()), true;
+#define MFL_LN(L_, V_, N_)                                                                                   \
+  if (H <= L_ * V_ * N_) {                                                                                   \
+    auto g = [&](auto exact) {                                                                               \
+      f(std::integral_constant<int, L_>(), std::integral_constant<int, V_>(), std::integral_constant<int, N_>(), exact); \
+    };                                                                                                       \
+    if (H == L_ * V_ * N_) g(std::true_type());                                                              \
+    else g(std::false_type());                                                                               \
+    return true;                                                                                             \
+  }
   if (H < N) {
     MFL_LN(16, 1, 1)
   }
   MFL_LN(16, 1, N)
-  MFL_LN(64, 1, N) MFL_LN(64, 2, N)
+  if constexpr (N == 8) {
+    MFL_LN(64, 1, 4)
+  }
+  MFL_LN(64, 1, N)
+  if constexpr (N == 8) {
+    MFL_LN(64, 3, 4)
+  }
+  MFL_LN(64, 2, N)
   if constexpr (N == 4 && !BACK) {  // (backward: 32 registers of loads ahead are too many)
-    MFL_LN(64, 4, N)
+    MFL_LN(64, 3, N) MFL_LN(64, 4, N)
   }
   MFL_LN(256, 1, N) MFL_LN(256, 2, N)
   if constexpr (N == 4) {
     MFL_LN(256, 4, N)
+  }
+  if constexpr (N == 8 && !BACK) {
+    MFL_LN(256, 3, N)
   }
   MFL_LN(1024, 1, N) MFL_LN(1024, 2, N)
   if constexpr (N == 4) {
@@ -409,10 +440,10 @@ constexpr int bwd_block(int lanes) { return lanes == 256 ? 256 : 1024; }
 
 template <typename T, typename P>
 void fwd_typed(const LayerNormFwd& a, hipStream_t s) {
-  const bool done = with_shape<T, false>(a.H, [&](auto L, auto V, auto N) {
+  const bool done = with_shape<T, false>(a.H, [&](auto L, auto V, auto N, auto exact) {
     constexpr int BLOCK = fwd_block(L), ROWS = BLOCK / L;
     const int64_t want = ((int64_t)a.M + ROWS - 1) / ROWS, cap = 2048 * 256 / BLOCK;
-    ln_fwd_kernel<T, P, BLOCK, L, V, N><<<(unsigned)(want < cap ? want : cap), BLOCK, 0, s>>>(a);
+    ln_fwd_kernel<T, P, BLOCK, L, V, N, exact><<<(unsigned)(want < cap ? want : cap), BLOCK, 0, s>>>(a);
   });
   if (!done) ln_fwd_long_kernel<T, P><<<(unsigned)(a.M < (1 << 20) ? a.M : (1 << 20)), 1024, 0, s>>>(a);
 }
@@ -422,7 +453,7 @@ void fwd_typed(const LayerNormFwd& a, hipStream_t s) {
 template <typename T>
 int bwd_blocks(int M, int H) {
   int G = M < 64 ? M : 64;
-  with_shape<T, true>(H, [&](auto L, auto, auto) {
+  with_shape<T, true>(H, [&](auto L, auto, auto, auto) {
     constexpr int BLOCK = bwd_block(L), ROWS = BLOCK / L;
     const int want = (int)(((int64_t)M + ROWS - 1) / ROWS), cap = BLOCK == 1024 ? 256 : 512;
     G = want < cap ? want : cap;
@@ -433,9 +464,9 @@ int bwd_blocks(int M, int H) {
 template <typename T, typename P>
 void bwd_typed(const LayerNormBwd& a, hipStream_t s) {
   const int G = bwd_blocks<T>(a.M, a.H);
-  const bool done = with_shape<T, true>(a.H, [&](auto L, auto V, auto N) {
+  const bool done = with_shape<T, true>(a.H, [&](auto L, auto V, auto N, auto exact) {
     constexpr int BLOCK = bwd_block(L);
-    ln_bwd_kernel<T, P, BLOCK, L, V, N><<<G, BLOCK, 0, s>>>(a);
+    ln_bwd_kernel<T, P, BLOCK, L, V, N, exact><<<G, BLOCK, 0, s>>>(a);
   });
   if (!done) {
     ln_bwd_long_kernel<T, P><<<(unsigned)(a.M < (1 << 20) ? a.M : (1 << 20)), 1024, 0, s>>>(a);
