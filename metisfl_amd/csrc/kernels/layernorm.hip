@@ -224,7 +224,7 @@ __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
   constexpr int WIDE = LANES * VPL * N;  // columns the registers of a row's lanes hold
   static_assert(LANES <= 64 || ROWS == 1, "a barrier belongs to one row");
   __shared__ float lds[2][32];
-  __shared__ float sums[ROWS > 1 ? ROWS / 2 * WIDE : 1];
+  __shared__ float sums[ROWS > 1 ? ROWS * WIDE : 1];
   const int lane = threadIdx.x % LANES, grp = row_group<LANES>();
   const Columns<LANES, VPL, N, EXACT> at(lane, a.H);
   const float inv = 1.f / (float)a.H;
@@ -284,36 +284,23 @@ __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
     store_packs<T>(static_cast<T*>(a.dx) + row * a.H, at, u);
   }
   if (!a.part) return;
-  // one row of partial sums for the workgroup: dgamma, then dbeta; the groups
-  // halve until one is left
+  // one row of partial sums for the workgroup: dgamma, then dbeta, the groups'
+  // added by column
   for (int which = 0; which < 2; ++which) {
-    float(&mine)[VPL][N] = which ? db : dg;
-    if constexpr (ROWS > 1) {
-#pragma unroll
-      for (int half = ROWS / 2; half > 0; half /= 2) {
-        __syncthreads();
-        if (grp >= half && grp < 2 * half) {
-#pragma unroll
-          for (int i = 0; i < VPL; ++i)
-#pragma unroll
-            for (int k = 0; k < N; ++k) sums[(grp - half) * WIDE + (k * VPL + i) * LANES + lane] = mine[i][k];
-        }
-        __syncthreads();
-        if (grp < half) {
-#pragma unroll
-          for (int i = 0; i < VPL; ++i)
-#pragma unroll
-            for (int k = 0; k < N; ++k) mine[i][k] += sums[grp * WIDE + (k * VPL + i) * LANES + lane];
-        }
-      }
-    }
+    const float(&mine)[VPL][N] = which ? db : dg;
     float* out = a.part + ((int64_t)blockIdx.x * 2 + which) * a.H;
-    if (grp == 0) {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          if (at.has(i, k)) out[at.c[i] + k] = mine[i][k];
+    if constexpr (ROWS == 1) {
+      store_packs<float>(out, at, mine);
+    } else {
+      if (which) __syncthreads();
+      store_packs<float>(sums + grp * WIDE, at, mine);
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.H; c += BLOCK) {
+        float s = 0.f;
+#pragma unroll 16
+        for (int r = 0; r < ROWS; ++r) s += sums[r * WIDE + c];
+        out[c] = s;
+      }
     }
   }
 }
@@ -397,29 +384,38 @@ __global__ __launch_bounds__(1024) void ln_wgrad_kernel(const float* __restrict_
 template <typename T, bool BACK, typename F>
 bool with_shape(int H, F&& f) {
   constexpr int N = Vec<T>::N;
-#define MFL_LN(L_, V_, N_)                                                                                   \
-  if (H <= L_ * V_ * N_) {                                                                                   \
-    auto g = [&](auto exact) {                                                                               \
-      f(std::integral_constant<int, L_>(), std::integral_constant<int, V_>(), std::integral_constant<int, N_>(), exact); \
-    };                                                                                                       \
-    if (H == L_ * V_ * N_) g(std::true_type());                                                              \
-    else g(std::false_type());                                                                               \
-    return true;                                                                                             \
-  }
+#define MFL_LN_EXACT(L_, V_, N_)                                                                           \
+  if (H == L_ * V_ * N_)                                                                                   \
+    return f(std::integral_constant<int, L_>(), std::integral_constant<int, V_>(),                         \
+             std::integral_constant<int, N_>(), std::true_type()), true;
+#define MFL_LN_UP_TO(L_, V_, N_)                                                                           \
+  if (H <= L_ * V_ * N_)                                                                                   \
+    return f(std::integral_constant<int, L_>(), std::integral_constant<int, V_>(),                         \
+             std::integral_constant<int, N_>(), std::false_type()), true;
+#define MFL_LN(L_, V_, N_) MFL_LN_EXACT(L_, V_, N_) MFL_LN_UP_TO(L_, V_, N_)
   if (H < N) {
-    MFL_LN(16, 1, 1)
+    MFL_LN_UP_TO(16, 1, 1)
   }
   MFL_LN(16, 1, N)
-  if constexpr (N == 8) {
-    MFL_LN(64, 1, 4)
+  if constexpr (N == 4 || !BACK) {
+    MFL_LN(16, 2, N)
+  } else {
+    MFL_LN_EXACT(16, 2, N)  // (masks are registers too many)
+    MFL_LN_UP_TO(64, 1, 4)
+  }
+  if constexpr (N == 4 && !BACK) {
+    MFL_LN(16, 4, N)
   }
   MFL_LN(64, 1, N)
   if constexpr (N == 8) {
     MFL_LN(64, 3, 4)
   }
   MFL_LN(64, 2, N)
+  if constexpr (N == 4) {
+    MFL_LN(64, 3, N)
+  }
   if constexpr (N == 4 && !BACK) {  // (backward: 32 registers of loads ahead are too many)
-    MFL_LN(64, 3, N) MFL_LN(64, 4, N)
+    MFL_LN(64, 4, N)
   }
   MFL_LN(256, 1, N) MFL_LN(256, 2, N)
   if constexpr (N == 4) {
@@ -433,6 +429,8 @@ bool with_shape(int H, F&& f) {
     MFL_LN(1024, 4, N)
   }
 #undef MFL_LN
+#undef MFL_LN_UP_TO
+#undef MFL_LN_EXACT
   return false;
 }
 constexpr int fwd_block(int lanes) { return lanes > 256 ? lanes : 256; }
