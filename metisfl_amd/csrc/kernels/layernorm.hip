@@ -183,24 +183,41 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LayerNormFwd a) {
   }
 }
 
-// Rows wider than registers hold: 1024 threads read the row three times (the
-// later two from L2).
+// Rows wider than registers hold: f(c, n, elements) for the n = N elements from
+// column c of each whole pack of this thread, then for single ones behind them.
+template <int N, typename F>
+__device__ __forceinline__ void each_pack(int H, F&& f) {
+  const int packs = H / N;
+  for (int i = threadIdx.x; i < packs; i += 1024) f(i * N, std::integral_constant<int, N>());
+  if (packs * N + (int)threadIdx.x < H) f(packs * N + (int)threadIdx.x, std::integral_constant<int, 1>());
+}
+
+// 1024 threads read such a row three times (the later two from L2).
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LayerNormFwd a) {
+  constexpr int N = Vec<T>::N;
   __shared__ float lds[2][32];
   const float width = (float)a.H;
   for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     float s = 0.f, zero = 0.f;
-    for (int c = threadIdx.x; c < a.H; c += 1024) s += to_f(x[c]);
+    each_pack<N>(a.H, [&](int c, auto n) {
+      const auto v = load_pack<T, n>(x + c);
+#pragma unroll
+      for (int k = 0; k < n; ++k) s += to_f(v.e[k]);
+    });
     row_sum2<1024>(s, zero, lds[0]);
     const float mean = s / width;
     float q = 0.f, rest = 0.f;
-    for (int c = threadIdx.x; c < a.H; c += 1024) {
-      const float d = to_f(x[c]) - mean;
-      q = fmaf(d, d, q);
-      rest += d;
-    }
+    each_pack<N>(a.H, [&](int c, auto n) {
+      const auto v = load_pack<T, n>(x + c);
+#pragma unroll
+      for (int k = 0; k < n; ++k) {
+        const float d = to_f(v.e[k]) - mean;
+        q = fmaf(d, d, q);
+        rest += d;
+      }
+    });
     row_sum2<1024>(q, rest, lds[1]);
     rest /= width;
     const float rstd = row_rstd(q / width, rest, a.eps);
@@ -210,11 +227,18 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LayerNormFwd a) {
       a.rstd[row] = rstd;
     }
     T* y = static_cast<T*>(a.y) + row * a.H;
-    for (int c = threadIdx.x; c < a.H; c += 1024) {
-      const float g = a.gamma ? to_f(static_cast<const P*>(a.gamma)[c]) : 1.f;
-      const float b = a.beta ? to_f(static_cast<const P*>(a.beta)[c]) : 0.f;
-      y[c] = from_f<T>((to_f(x[c]) - mean - rest) * rstd * g + b);
-    }
+    each_pack<N>(a.H, [&](int c, auto n) {
+      const auto v = load_pack<T, n>(x + c);
+      Pack<P, n> g, b;
+      if (a.gamma) g = load_pack<P, n>(static_cast<const P*>(a.gamma) + c);
+      if (a.beta) b = load_pack<P, n>(static_cast<const P*>(a.beta) + c);
+      Pack<T, n> o;
+#pragma unroll
+      for (int k = 0; k < n; ++k)
+        o.e[k] = from_f<T>((to_f(v.e[k]) - mean - rest) * rstd * (a.gamma ? to_f(g.e[k]) : 1.f) +
+                           (a.beta ? to_f(b.e[k]) : 0.f));
+      store_pack<T, n>(y + c, o);
+    });
   }
 }
 
@@ -305,43 +329,70 @@ __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
   }
 }
 
-// Rows wider than registers hold: a workgroup takes a row at a time for dx,
-// and the weights' gradients are column sums in launches of their own.
+// Rows wider than registers hold: a workgroup takes a row at a time for dx
+// (read twice), and the weights' gradients are column sums in launches of
+// their own.
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(LayerNormBwd a) {
+  constexpr int N = Vec<T>::N;
   __shared__ float lds[2][32];
   const float inv = 1.f / (float)a.H;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x, turn ^= 1) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+    T* dx = static_cast<T*>(a.dx) + row * a.H;
     const float mean = a.mean[row], rstd = a.rstd[row];
     float s1 = 0.f, s2 = 0.f;
-    for (int c = threadIdx.x; c < a.H; c += 1024) {
-      const float u = to_f(dy[c]) * (a.gamma ? to_f(static_cast<const P*>(a.gamma)[c]) : 1.f);
-      s1 += u;
-      s2 += u * ((to_f(x[c]) - mean) * rstd);
-    }
+    auto pass = [&](auto write) {
+      each_pack<N>(a.H, [&](int c, auto n) {
+        const auto v = load_pack<T, n>(x + c);
+        const auto d = load_pack<T, n>(dy + c);
+        Pack<P, n> g;
+        if (a.gamma) g = load_pack<P, n>(static_cast<const P*>(a.gamma) + c);
+        Pack<T, n> o;
+#pragma unroll
+        for (int k = 0; k < n; ++k) {
+          const float xh = (to_f(v.e[k]) - mean) * rstd, u = to_f(d.e[k]) * (a.gamma ? to_f(g.e[k]) : 1.f);
+          if constexpr (write) {
+            o.e[k] = from_f<T>(rstd * (u - s1 - xh * s2));
+          } else {
+            s1 += u;
+            s2 += u * xh;
+          }
+        }
+        if constexpr (write) store_pack<T, n>(dx + c, o);
+      });
+    };
+    pass(std::false_type());
     row_sum2<1024>(s1, s2, lds[turn]);
     s1 *= inv;
     s2 *= inv;
-    T* dx = static_cast<T*>(a.dx) + row * a.H;
-    for (int c = threadIdx.x; c < a.H; c += 1024) {
-      const float u = to_f(dy[c]) * (a.gamma ? to_f(static_cast<const P*>(a.gamma)[c]) : 1.f);
-      dx[c] = from_f<T>(rstd * (u - s1 - (to_f(x[c]) - mean) * rstd * s2));
-    }
+    pass(std::true_type());
   }
 }
-// partials of 256 columns (blockIdx.x) over every gridDim.y-th row
+// partials of 256 columns (blockIdx.x) over every gridDim.y-th row, four rows' loads in flight
 template <typename T>
 __global__ __launch_bounds__(256) void ln_colsum_long_kernel(LayerNormBwd a) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= a.H) return;
   float dg = 0.f, db = 0.f;
-  for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
-    const float d = to_f(static_cast<const T*>(a.dy)[row * a.lddy + c]);
-    dg += d * ((to_f(static_cast<const T*>(a.x)[row * a.ldx + c]) - a.mean[row]) * a.rstd[row]);
-    db += d;
+  for (int64_t row = blockIdx.y; row < a.M; row += 4 * (int64_t)gridDim.y) {
+    float d[4], x[4], mean[4], rstd[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = row + j * (int64_t)gridDim.y, r = at < a.M ? at : a.M - 1;
+      d[j] = to_f(static_cast<const T*>(a.dy)[r * a.lddy + c]);
+      x[j] = to_f(static_cast<const T*>(a.x)[r * a.ldx + c]);
+      mean[j] = a.mean[r];
+      rstd[j] = a.rstd[r];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (row + j * (int64_t)gridDim.y >= a.M) break;
+      dg += d[j] * ((x[j] - mean[j]) * rstd[j]);
+      db += d[j];
+    }
   }
   a.part[((int64_t)blockIdx.y * 2) * a.H + c] = dg;
   a.part[((int64_t)blockIdx.y * 2 + 1) * a.H + c] = db;
