@@ -338,7 +338,7 @@ class AdamPlan {
     };
     table_ = upload(table.data(), table.size() * sizeof(table[0]));
     chunks_ = upload(list.data(), list.size() * sizeof(mfl::AdamChunk));
-    scalars_ = torch::empty({(int64_t)sizeof(mfl::AdamScalars)}, first.options().dtype(torch::kUInt8));
+    scalars_ = torch::zeros({(int64_t)sizeof(mfl::AdamScalars) + 4}, first.options().dtype(torch::kUInt8));
   }
 
   void step(const std::vector<OptTensor>& grads, double lr, double beta1, double beta2, double eps, int64_t seed) {
@@ -358,6 +358,7 @@ class AdamPlan {
     a.tensors = reinterpret_cast<const mfl::AdamTensor*>(table_.data_ptr());
     a.chunks = reinterpret_cast<const mfl::AdamChunk*>(chunks_.data_ptr());
     a.scalars = reinterpret_cast<mfl::AdamScalars*>(scalars_.data_ptr());
+    a.arrived = reinterpret_cast<int*>(a.scalars + 1);
     a.step = step_.data_ptr<int>();
     a.lr_scale = lr_scale_.defined() ? lr_scale_.data_ptr<float>() : nullptr;
     a.m = m_.data_ptr();
@@ -372,7 +373,8 @@ class AdamPlan {
     a.lr = (float)lr;
     a.seed = (uint32_t)seed;
     a.state_bits = bits_;
-    mfl::launch_adam_begin(a, s);
+    const bool whole = firsts_.size() == 2 && firsts_[1] > 0 && firsts_[1] <= mfl::kAdamWhole;
+    if (!whole) mfl::launch_adam_begin(a, s);
     C10_HIP_KERNEL_LAUNCH_CHECK();
     mfl::AdamGrads g;
     for (size_t part = 0; part + 1 < firsts_.size(); ++part) {
@@ -383,7 +385,7 @@ class AdamPlan {
         g.g[i - lo] = given(grads[i]) ? grads[i]->data_ptr() : nullptr;
         g.type[i - lo] = given(grads[i]) ? (uint8_t)elem_type(*grads[i], "a gradient") : 0;
       }
-      mfl::launch_adam_chunks(a, g, (int)lo, firsts_[part], n, s);
+      mfl::launch_adam_chunks(a, g, (int)lo, firsts_[part], n, whole, s);
       C10_HIP_KERNEL_LAUNCH_CHECK();
     }
   }

@@ -99,6 +99,7 @@ struct AdamStep {
   const AdamTensor* tensors;
   const AdamChunk* chunks;
   AdamScalars* scalars;
+  int* arrived;                    // zero between steps
   int* step;
   const float* lr_scale;           // or null
   void* m;
@@ -115,7 +116,10 @@ struct AdamGrads {                 // gradients of tensors first .. first + coun
   uint8_t type[kAdamGrads];
 };
 void launch_adam_begin(const AdamStep& a, hipStream_t s);
+// whole: these are all of the step's chunks, at most kAdamWhole, and the launch
+// does what launch_adam_begin would
+constexpr int kAdamWhole = 512;
 void launch_adam_chunks(const AdamStep& a, const AdamGrads& g, int first_tensor, int64_t first_chunk, int64_t chunks,
-                        hipStream_t s);
+                        bool whole, hipStream_t s);
 
 }  // namespace mfl
