@@ -8,6 +8,7 @@
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cstring>
 #include <limits>
 #include <vector>
 
@@ -331,20 +332,23 @@ class AdamPlan {
       vector_of(*lr_scale, first, torch::kFloat32, 1, "lr_scale");
       lr_scale_ = *lr_scale;
     }
-    auto upload = [&](const void* from, size_t bytes) {
-      Tensor host = torch::empty({(int64_t)std::max<size_t>(bytes, 1)}, torch::kUInt8);
-      if (bytes) memcpy(host.data_ptr(), from, bytes);
-      return host.to(first.device());
-    };
-    table_ = upload(table.data(), table.size() * sizeof(table[0]));
-    chunks_ = upload(list.data(), list.size() * sizeof(mfl::AdamChunk));
-    scalars_ = torch::zeros({(int64_t)sizeof(mfl::AdamScalars) + 4}, first.options().dtype(torch::kUInt8));
+    for (const mfl::AdamTensor& t : table) pointers_.push_back(t.p);
+    // one copy: the table, the chunks, and zeros for the scalars and the arrivals
+    const size_t tb = table.size() * sizeof(table[0]), cb = list.size() * sizeof(mfl::AdamChunk);
+    Tensor host = torch::zeros({(int64_t)(tb + cb + sizeof(mfl::AdamScalars) + sizeof(int))}, torch::kUInt8);
+    uint8_t* h = host.data_ptr<uint8_t>();
+    memcpy(h, table.data(), tb);
+    if (cb) memcpy(h + tb, list.data(), cb);
+    chunks_at_ = tb;
+    scalars_at_ = tb + cb;
+    tables_ = host.to(first.device());
   }
 
   void step(const std::vector<OptTensor>& grads, double lr, double beta1, double beta2, double eps, int64_t seed) {
     const Tensor& first = params_[0];
     TORCH_CHECK(grads.size() == params_.size(), "got ", grads.size(), " gradients for ", params_.size(), " parameters");
     for (size_t i = 0; i < grads.size(); ++i) {
+      TORCH_CHECK(params_[i].data_ptr() == pointers_[i], "parameter ", i, " has another storage than at construction");
       if (!given(grads[i])) continue;
       const Tensor& g = *grads[i];
       same_device(g, first, "a gradient");
@@ -355,9 +359,10 @@ class AdamPlan {
     c10::DeviceGuard guard(first.device());
     const hipStream_t s = stream_of(first);
     mfl::AdamStep a{};
-    a.tensors = reinterpret_cast<const mfl::AdamTensor*>(table_.data_ptr());
-    a.chunks = reinterpret_cast<const mfl::AdamChunk*>(chunks_.data_ptr());
-    a.scalars = reinterpret_cast<mfl::AdamScalars*>(scalars_.data_ptr());
+    uint8_t* tables = tables_.data_ptr<uint8_t>();
+    a.tensors = reinterpret_cast<const mfl::AdamTensor*>(tables);
+    a.chunks = reinterpret_cast<const mfl::AdamChunk*>(tables + chunks_at_);
+    a.scalars = reinterpret_cast<mfl::AdamScalars*>(tables + scalars_at_);
     a.arrived = reinterpret_cast<int*>(a.scalars + 1);
     a.step = step_.data_ptr<int>();
     a.lr_scale = lr_scale_.defined() ? lr_scale_.data_ptr<float>() : nullptr;
@@ -393,7 +398,9 @@ class AdamPlan {
  private:
   std::vector<Tensor> params_;
   std::vector<OptTensor> mirrors_;
-  Tensor m_, v_, m_scale_, v_scale_, step_, lr_scale_, table_, chunks_, scalars_;
+  Tensor m_, v_, m_scale_, v_scale_, step_, lr_scale_, tables_;
+  std::vector<void*> pointers_;  // the parameters' storage, as the table has it
+  size_t chunks_at_ = 0, scalars_at_ = 0;
   std::vector<int64_t> firsts_;  // first chunk of each launch's tensors, and the end
   int bits_ = 32;
 };

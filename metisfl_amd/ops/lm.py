@@ -46,6 +46,10 @@ def _check_norm(x, gamma, beta):
     for nm, p in (("gamma", gamma), ("beta", beta)):
         if p is not None and tuple(p.shape) != (x.shape[-1],):
             raise ValueError(f"{nm} has shape {tuple(p.shape)}, expected ({x.shape[-1]},)")
+        if p is not None and p.dtype not in (torch.float32, x.dtype):
+            raise RuntimeError(f"{nm} must be float32 or of the input's type, got {p.dtype}")
+    if beta is not None and beta.dtype != gamma.dtype:
+        raise RuntimeError("gamma and beta must have the same type")
 
 
 def layer_norm_fwd(x, gamma=None, beta=None, eps: float = 1e-5):

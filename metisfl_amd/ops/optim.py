@@ -150,12 +150,14 @@ STATE_BLOCK = 128  # elements that share a scale of MultiTensorAdamW's 8-bit sta
 
 
 class MultiTensorAdamW:
-    """Adam / AdamW over a list of tensors, the whole step in two launches (one
-    more for each further 384 tensors; csrc/kernels/multi_adamw.hip).
+    """Adam / AdamW over a list of tensors, the whole step in one launch (up to a
+    million elements) or two, and one more for each further 384 tensors
+    (csrc/kernels/multi_adamw.hip).
 
     ``params``: contiguous float32 or bfloat16 tensors on one device, updated
-    in place; they keep their storage for the optimizer's life.  ``decay``:
-    which of them take ``spec.weight_decay`` (default: all).  ``mirrors``: a
+    in place, no two of them sharing memory; they keep their storage for the
+    optimizer's life (a step refuses one that was moved).  ``decay``: which of
+    them take ``spec.weight_decay`` (default: all).  ``mirrors``: a
     bfloat16 copy of each parameter (or None) that the step refreshes.
     ``lr_scale``: a float32 device tensor of one element that the step
     multiplies the learning rate with.
@@ -193,6 +195,10 @@ class MultiTensorAdamW:
             if q is not None and (q.dtype != torch.bfloat16 or not q.is_contiguous() or q.device != dev
                                   or q.numel() != p.numel()):
                 raise ValueError("a mirror must be a contiguous bfloat16 tensor of its parameter's size and device")
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                       for t in self.params + self.mirrors if t is not None and t.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("parameters and mirrors must not share memory (list a tied weight once)")
         wd = spec.weight_decay if spec.mode == OPT_ADAMW else 0.0
         self.weight_decays = [wd if d else 0.0 for d in decay]
         self.offsets, total = [], 0
@@ -208,12 +214,10 @@ class MultiTensorAdamW:
         self.step_count = zeros(1, torch.int32)
         self.lr_scale = lr_scale
         self._plan = None
+        self._pointers = [p.data_ptr() for p in self.params]
         if dev.type == "cuda":
-            self._plan = ops().AdamPlan(self._storages(), self.mirrors, self.weight_decays, self.m, self.v,
+            self._plan = ops().AdamPlan(self.params, self.mirrors, self.weight_decays, self.m, self.v,
                                         self.m_scale, self.v_scale, self.step_count, lr_scale, self.offsets)
-
-    def _storages(self) -> list[torch.Tensor]:
-        return [p.detach() for p in self.params]
 
     @torch.no_grad()
     def step(self, grads=None) -> None:
@@ -253,7 +257,9 @@ class MultiTensorAdamW:
     def _reference(self, grads) -> None:
         if len(grads) != len(self.params):
             raise ValueError(f"got {len(grads)} gradients for {len(self.params)} parameters")
-        for p, g in zip(self.params, grads):
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if p.data_ptr() != self._pointers[i]:
+                raise ValueError(f"parameter {i} has another storage than at construction")
             if g is None:
                 continue
             if g.dtype not in (torch.float32, torch.bfloat16, torch.float16) or not g.is_contiguous() \

@@ -53,6 +53,10 @@ def test_layer_norm_refusals():
         lm.layer_norm_fwd(x, None, torch.ones(4))
     with pytest.raises(ValueError, match="no elements"):
         lm.layer_norm_fwd(torch.zeros(2, 0))
+    with pytest.raises(RuntimeError, match="input's type"):
+        lm.layer_norm_fwd(x, torch.ones(4, dtype=torch.float16))
+    with pytest.raises(RuntimeError, match="same type"):
+        lm.layer_norm_fwd(x.half(), torch.ones(4), torch.ones(4, dtype=torch.float16))
     with pytest.raises(ValueError, match="dy"):
         lm.layer_norm_bwd(torch.zeros(2, 3), x, torch.zeros(2), torch.ones(2))
 
@@ -236,6 +240,16 @@ def test_adamw_refusals():
         MultiTensorAdamW(SPEC, p, mirrors=[torch.zeros(4)])
     with pytest.raises(ValueError, match="one entry"):
         MultiTensorAdamW(SPEC, p, decay=[True, False])
+    with pytest.raises(ValueError, match="share memory"):
+        MultiTensorAdamW(SPEC, [p[0], p[0]])
+    flat = torch.zeros(10)
+    with pytest.raises(ValueError, match="share memory"):
+        MultiTensorAdamW(SPEC, [flat[:6], flat[5:]])
+    moved = [torch.zeros(4)]
+    opt = MultiTensorAdamW(SPEC, moved)
+    moved[0].data = torch.ones(4)
+    with pytest.raises(ValueError, match="another storage"):
+        opt.step([torch.zeros(4)])
     opt = MultiTensorAdamW(SPEC, p)
     with pytest.raises(ValueError, match="gradient"):
         opt.step([torch.zeros(5)])
@@ -294,7 +308,7 @@ def check_step_gradients(device):
     net = net.to(device)
     loss = loss_of(net(tokens.to(device)), targets.to(device))
     loss.backward()
-    assert abs(float(loss) - float(ref)) < 1e-5
+    assert abs(float(loss.detach()) - float(ref.detach())) < 1e-5
     for (n, p), q in zip(net.named_parameters(), want.parameters()):
         # fp32 sums of up to 50 x 36 products
         torch.testing.assert_close(p.grad.cpu().double(), q.grad, rtol=1e-4, atol=1e-5 * float(q.grad.abs().max()), msg=n)

@@ -73,7 +73,7 @@ def test_layer_norm_widths(t, h):
         check_norm(x, gamma, beta, 1e-5, dy)
 
 
-@pytest.mark.parametrize("rows,h", [(5000, 256), (16384, 24), (4099, 768), (2049, 2304), (1031, 5120), (3000, 40)])
+@pytest.mark.parametrize("rows,h", [(5000, 256), (70000, 24), (4099, 768), (2049, 2304), (1031, 5120), (3000, 40)])
 @pytest.mark.parametrize("t", TYPES)
 def test_layer_norm_many_rows(t, rows, h):
     g = gen(rows)
@@ -326,6 +326,30 @@ def test_token_logprobs_autograd():
     torch.testing.assert_close(b.grad, c.grad, rtol=1e-4, atol=1e-7)
 
 
+def test_token_logprobs_many_rows():
+    """More rows than one launch has workgroups."""
+    g = gen(8)
+    z = torch.randn(4_300_000, 4, generator=g, device=DEV)
+    target = torch.randint(-1, 4, (z.shape[0],), generator=g, device=DEV)
+    check_logprobs(z, target, 2, 4)
+
+
+def test_token_logprobs_gradient_of_repeated_ids():
+    """Alternatives that name the same token, or the target, add up."""
+    z, target = make_logits(3, 5000, 5000, torch.float32, 9)
+    target = torch.tensor([7, 4999, -1], device=DEV)
+    ids = torch.tensor([[7, 7, 3], [4999, 0, 4999], [11, 11, 11]], device=DEV)
+    r = lm.token_logprobs_fwd(z, target, 0)
+    d_logp, d_top = torch.tensor([1.0, 2.0, 3.0], device=DEV), torch.arange(1.0, 10.0, device=DEV).view(3, 3)
+    dx = lm.token_logprobs_bwd(z, target, r.stats, d_logp, None, d_top, ids)
+    p = torch.softmax(z.double(), -1)
+    w = d_logp.double() * (target >= 0)
+    want = -p * (w + d_top.double().sum(1))[:, None]
+    want.scatter_add_(1, ids, d_top.double())
+    want.scatter_add_(1, target.clamp(min=0)[:, None], w[:, None])
+    near(dx, want, 1e-5 * want.abs() + 1e-6 * p, "dlogits")
+
+
 def test_token_logprobs_refusals():
     z, t = torch.zeros(2, 9, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
     with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
@@ -480,6 +504,11 @@ def test_adamw_refusals():
     with pytest.raises(RuntimeError, match="gradients"):
         opt.step([])
     assert int(opt.step_count) == 0  # a refused step changes nothing
+    moved = torch.zeros(8, device=DEV)
+    opt = MultiTensorAdamW(SPEC, [moved])
+    moved.data = torch.ones(8, device=DEV)
+    with pytest.raises(RuntimeError, match="another storage"):
+        opt.step([torch.zeros(8, device=DEV)])
     with pytest.raises(RuntimeError, match="lr_scale"):
         MultiTensorAdamW(SPEC, p, lr_scale=torch.ones(1))
 
@@ -535,6 +564,36 @@ def test_static_step_in_two_graphs(rows, width, vocab):
         for args, graph, out, side in steps:
             for a, b in zip(out, static_step(*args)):
                 assert torch.equal(a, b)
+
+
+def test_autograd_in_a_graph():
+    """Both operators and their backwards captured, replayed against eager."""
+    g = gen(15)
+    x = torch.randn(40, 3001, generator=g, device=DEV)
+    target = torch.randint(0, 3001, (40,), generator=g, device=DEV)
+    weight = torch.rand(40, generator=g, device=DEV)
+
+    def grads():
+        a = x.detach().requires_grad_()
+        w = torch.ones(3001, device=DEV, requires_grad=True)
+        b = torch.zeros(3001, device=DEV, requires_grad=True)
+        r = lm.token_logprobs(lm.layer_norm(a, w, b), target, 3)
+        return torch.autograd.grad((r.logp, r.entropy), (a, w, b), (weight, weight))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = grads()
+    for k in range(3):
+        x.normal_(0.0, 1.0 + k, generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, grads()):
+            assert torch.equal(p, q)
 
 
 def test_results_on_another_stream():
