@@ -50,6 +50,17 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& v) {
   __builtin_memcpy(p, &v, sizeof(v));
 }
 
+// The same past the caches' write-back (16 bytes): for results that nothing
+// reads soon, a stream of stores then does not fetch or evict lines.
+template <typename T, int N>
+__device__ __forceinline__ void stream_pack(T* p, const Pack<T, N>& v) {
+  typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+  static_assert(sizeof(v) == 16, "16 bytes");
+  Words w;
+  __builtin_memcpy(&w, &v, sizeof(w));
+  __builtin_nontemporal_store(w, reinterpret_cast<Words*>(p));
+}
+
 // Reductions over a wave's rows of 16 lanes by DPP rotations (every lane gets
 // the result; a rotation costs a VALU instruction where a shuffle goes through
 // LDS), and over all 64 lanes by four lane reads more.  The lanes of a row (of
