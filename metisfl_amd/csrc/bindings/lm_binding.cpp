@@ -77,6 +77,25 @@ int param_type(const Tensor& p, const Tensor& x, int64_t H, const char* nm) {
   return t;
 }
 
+// Small results of a call come from one allocation (each costs the host a
+// microsecond, which is a fifth of a call on one token).
+class Results {
+ public:
+  Results(int64_t elements, const c10::TensorOptions& o) : all_(at::empty({elements}, o)) {}
+  Tensor next(c10::IntArrayRef sizes) {
+    auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(all_.storage()), all_.key_set(), all_.dtype());
+    t->set_sizes_contiguous(sizes);
+    t->set_storage_offset(at_);
+    at_ += t->numel();
+    TORCH_INTERNAL_ASSERT(at_ <= all_.numel());
+    return Tensor(std::move(t));
+  }
+
+ private:
+  Tensor all_;
+  int64_t at_ = 0;
+};
+
 c10::IntArrayRef lead_of(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
 
 void norm_weights(const Tensor& x, int64_t H, const OptTensor& gamma, const OptTensor& beta) {
@@ -103,8 +122,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x, const OptTens
     TORCH_CHECK(param_type(*beta, x, r.cols, "beta") == a.param_type, "gamma and beta must have the same type");
     a.beta = beta->data_ptr();
   }
-  const auto f32 = x.options().dtype(torch::kFloat32);
-  Tensor y = at::empty(x.sizes(), x.options()), mean = at::empty(lead_of(x), f32), rstd = at::empty(lead_of(x), f32);
+  Results small(2 * r.rows, x.options().dtype(torch::kFloat32));
+  Tensor y = at::empty(x.sizes(), x.options()), mean = small.next(lead_of(x)), rstd = small.next(lead_of(x));
   if (r.rows == 0) return {y, mean, rstd};
   a.x = r.p;
   a.y = y.data_ptr();
@@ -135,10 +154,17 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_bwd(const Tensor& dy, const 
   Tensor dx = at::empty(x.sizes(), x.options());
   OptTensor dgamma, dbeta;
   if (given(gamma)) {
-    dgamma = r.rows ? at::empty({r.cols}, gamma->options()) : at::zeros({r.cols}, gamma->options());
-    dbeta = r.rows ? at::empty({r.cols}, gamma->options()) : at::zeros({r.cols}, gamma->options());
+    Results small(2 * r.cols, gamma->options());
+    dgamma = small.next({r.cols});
+    dbeta = small.next({r.cols});
   }
-  if (r.rows == 0) return {dx, dgamma, dbeta};
+  if (r.rows == 0) {
+    if (given(gamma)) {
+      dgamma->zero_();
+      dbeta->zero_();
+    }
+    return {dx, dgamma, dbeta};
+  }
   Tensor part;  // the workgroups' partial sums, from the allocator of the current stream (or of a capture)
   a.dy = d.p;
   a.x = r.p;
@@ -197,11 +223,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_fwd(const Tens
   a.type = elem_type(x, "logits");
   const auto f32 = x.options().dtype(torch::kFloat32);
   auto shape = lead_of(x).vec();
-  Tensor logp = at::empty(shape, f32), entropy = at::empty(shape, f32);
+  Results small(r.rows * (5 + K), f32);
+  Tensor logp = small.next(shape), entropy = small.next(shape);
   shape.push_back(3);
-  Tensor stats = at::empty(shape, f32);
+  Tensor stats = small.next(shape);
   shape.back() = K;
-  Tensor top = at::empty(shape, f32), ids = at::empty(shape, x.options().dtype(torch::kInt64));
+  Tensor top = small.next(shape), ids = at::empty(shape, x.options().dtype(torch::kInt64));
   if (r.rows == 0) return {logp, entropy, top, ids, stats};
   Tensor work;  // parts of split rows, from the allocator of the current stream (or of a capture)
   if (const size_t bytes = mfl::token_logprobs_workspace((int)r.rows, (int)V, (int)K, a.type)) {
