@@ -35,12 +35,34 @@
 namespace mfl {
 namespace {
 
-__device__ __forceinline__ uint32_t mix32(uint32_t x) {
-  x *= 0x9E3779B1u;  // 2^32 / golden ratio, odd
+__device__ __forceinline__ uint32_t mix32_rest(uint32_t x) {
   x ^= x >> 15;
   x *= 0x6A09E667u;  // fraction of sqrt(2)
+  asm("" : "+v"(x));  // one product: a shift of it by 16 is not to become a second one
   return x ^ (x >> 16);
 }
+__device__ __forceinline__ uint32_t mix32(uint32_t x) { return mix32_rest(x * 0x9E3779B1u); }  // 2^32 / golden ratio, odd
+
+// Correctly rounded root and quotient in the range where their residuals are
+// exact (normal numbers of 2^-100 to 2^100): one Newton step on v_rsq_f32 with
+// the residual x - g^2 by a fused multiply-add, and Markstein's quotient
+// correction with a correctly rounded reciprocal.  The root and the reciprocal
+// were compared with 64 bits for every one of the 2^24 significands (root:
+// both parities of the exponent), the quotient for 8.6e9 pairs: none differs.
+// They take 8 and 9 issue slots where the general forms, which also scale, take
+// 19 and 15; the 8-bit step is bound by these as much as by memory (83 ragged
+// bf16 tensors 60 -> 57 us).
+__device__ __forceinline__ float root_in_range(float x) {
+  const float y = __builtin_amdgcn_rsqf(x), g = x * y;
+  return fmaf(fmaf(-g, g, x), 0.5f * y, g);
+}
+__device__ __forceinline__ float quotient_in_range(float n, float d) {
+  float r = __builtin_amdgcn_rcpf(d);
+  r = fmaf(fmaf(-d, r, 1.f), r, r);
+  const float q = n * r;
+  return fmaf(fmaf(-d, q, n), r, q);
+}
+constexpr uint32_t kLow = (127u - 100u) << 23, kHigh = (127u + 100u) << 23;  // magnitudes of 2^-100, 2^100
 
 // b^t by squaring, in 64 bits
 __device__ double power(double b, uint32_t t) {
@@ -112,6 +134,18 @@ __device__ __forceinline__ void unpack_states(uint2 w, float scale, float* f) {
   }
 }
 
+constexpr uint32_t kInf = 0x7f800000u;
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {  // over a row of 16 lanes
+#define MFL_ROR(N_) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N_, 0xf, 0xf, false))
+  MFL_ROR(8);
+  MFL_ROR(4);
+  MFL_ROR(2);
+  MFL_ROR(1);
+#undef MFL_ROR
+  return v;
+}
+
 // Codes of 8 values and their block's 2^E (16 threads, a row of the wave, have
 // a block).  The conversion with a dither adds the dither's high bits to those
 // a code drops, below 2^-6 too, where codes are 2^-9 apart; HIGH picks the half
@@ -119,18 +153,18 @@ __device__ __forceinline__ void unpack_states(uint2 w, float scale, float* f) {
 // become NaN and do not raise the scale.
 template <bool HIGH, bool LEAST>
 __device__ __forceinline__ uint2 pack_states(const float* x, const uint32_t* bits, float* scale) {
-  float top = 0.f;  // (the maximum passes over NaN)
+  uint32_t top = 0;  // magnitudes order as whole numbers, the non-finite ones on top
 #pragma unroll
-  for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
-  top = max16(top);
-  if (top == INFINITY) {
-    top = 0.f;
+  for (int k = 0; k < 8; ++k) top = max(top, magnitude(x[k]));
+  top = row_max(top);
+  if (top >= kInf) {
+    top = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = fabsf(x[k]) < INFINITY ? fmaxf(top, fabsf(x[k])) : top;
-    top = max16(top);
+    for (int k = 0; k < 8; ++k) top = magnitude(x[k]) < kInf ? max(top, magnitude(x[k])) : top;
+    top = row_max(top);
   }
   // biased exponent of 2^E: a block whose largest is below 2^-110 (or zero) takes the least
-  int e = (int)(__float_as_uint(top) >> 23) - 7;
+  int e = (int)(top >> 23) - 7;
   e = e < 10 ? 10 : e;
   *scale = __uint_as_float((uint32_t)e << 23);
   const float up = __uint_as_float((uint32_t)(254 - e) << 23);
@@ -230,16 +264,38 @@ __device__ __forceinline__ void adam_chunk(const AdamStep& a, const AdamTensor& 
       v[k] = in.v.e[k];
     }
   }
-  const int64_t at = at0 + i;
-  const uint32_t high = (uint32_t)(at >> 32) * 0x9E3779B1u;
+  uint32_t low = kHigh, high = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const float gk = to_f(in.g.e[k]), pk = to_f(in.p.e[k]);
+    const float gk = to_f(in.g.e[k]);
     m[k] = m[k] * b1 + gk * n1;
     v[k] = v[k] * b2 + (gk * n2) * gk;
-    r[k] = sqrtf(v[k]);
-    p[k] = pk - ((m[k] * sc.c1) / (r[k] * sc.c2 + a.eps) + pk * t.wd) * sc.lr;
-    if (BITS == 8 || sizeof(PT) == 2) bits[k] = mix32((((uint32_t)at + k) ^ sc.key) + high);
+    low = min(low, min(magnitude(v[k]), magnitude(m[k])));
+    high = max(high, max(magnitude(v[k]), magnitude(m[k])));
+  }
+  if (low >= kLow && high <= kHigh && magnitude(a.eps) <= kHigh) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      r[k] = root_in_range(v[k]);
+      p[k] = quotient_in_range(m[k] * sc.c1, r[k] * sc.c2 + a.eps);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      r[k] = sqrtf(v[k]);
+      p[k] = (m[k] * sc.c1) / (r[k] * sc.c2 + a.eps);
+    }
+  }
+  const int64_t at = at0 + i;
+  // mix32(((at + k) ^ key) + high part), its first product by parts: at is a
+  // multiple of 8, so (at + k) ^ key is (at ^ key with the low bits 0) + (k ^ the key's)
+  const uint32_t key = (uint32_t)__builtin_amdgcn_readfirstlane((int)sc.key);
+  const uint32_t base = (((uint32_t)at ^ (key & ~7u)) + (uint32_t)(at >> 32) * 0x9E3779B1u) * 0x9E3779B1u;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float pk = to_f(in.p.e[k]);
+    p[k] = pk - (p[k] + pk * t.wd) * sc.lr;
+    if (BITS == 8 || sizeof(PT) == 2) bits[k] = mix32_rest(base + (((uint32_t)k ^ key) & 7u) * 0x9E3779B1u);
   }
   if constexpr (BITS == 8) {
     float ms, vs;

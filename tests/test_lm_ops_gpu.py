@@ -412,6 +412,32 @@ def test_adamw_equals_the_reference(bits, ptypes, gtypes):
             same_bits(p, q)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("ptype", [torch.float32, torch.bfloat16])
+def test_adamw_equals_the_reference_at_all_magnitudes(bits, ptype):
+    """Gradients from 1e-38 to 1e18 and zeros, in one block and apart: roots and
+    quotients in and out of the range of the short forms."""
+    g = torch.Generator().manual_seed(21)
+    n = 128 * 40
+    mixed = torch.randn(n, generator=g) * 10.0 ** torch.randint(-38, 19, (n,), generator=g).float()
+    mixed[torch.rand(n, generator=g) < 0.2] = 0
+    apart = torch.randn(40, 128, generator=g) * 10.0 ** torch.arange(-30, 10).float()[:, None]
+    grads = [mixed, apart.reshape(-1).clone(), torch.zeros(200)]
+    params = [(torch.randn(x.numel(), generator=g) * 0.1).to(ptype) for x in grads]
+    params[2][:100] = 0
+    dev = [p.to(DEV) for p in params]
+    a = MultiTensorAdamW(SPEC, params, state_bits=bits, seed=5)
+    b = MultiTensorAdamW(SPEC, dev, state_bits=bits, seed=5)
+    for k in range(3):
+        gs = [x * (k + 1) for x in grads]
+        a.step(gs)
+        b.step([x.to(DEV) for x in gs])
+        for p, q in zip(params, dev):
+            same_bits(p, q)
+        for name, s in a.state_dict().items():
+            same_bits(s, b.state_dict()[name])
+
+
 def test_adamw_32_bits_against_definition():
     params, grads = make_tensors(SIZES, [torch.float32], [torch.float32], 2)
     dev = [p.to(DEV) for p in params]
