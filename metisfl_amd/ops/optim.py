@@ -171,8 +171,9 @@ class MultiTensorAdamW:
     step and place: equal seeds give equal results.  bfloat16 parameters are
     rounded the same way.  ``step_count`` is an int32 device tensor.
 
-    :meth:`step` can be captured into a hipGraph (with the gradients of the
-    captured backward)."""
+    :meth:`step` can be captured into a hipGraph with the gradients of the
+    captured backward; the graph keeps the spec's values (``lr_scale`` is read
+    by every replay)."""
 
     def __init__(self, spec: OptimizerSpec, params, *, state_bits: int = 32, decay=None, mirrors=None,
                  lr_scale: torch.Tensor | None = None, seed: int = 0):
