@@ -274,10 +274,7 @@ __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
 #pragma unroll
   for (int i = 0; i < VPL; ++i)
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      dg[i][k] = db[i][k] = 0.f;
-      if (!at.has(i, k)) g[i][k] = 0.f;  // another lane's element adds nothing to the row's sums
-    }
+    for (int k = 0; k < N; ++k) dg[i][k] = db[i][k] = 0.f;
   for (int turn = 0; row < a.M; row += step, turn ^= 1) {
     float xh[VPL][N], u[VPL][N];
 #pragma unroll
@@ -301,7 +298,7 @@ __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(LayerNormBwd a) {
       for (int k = 0; k < N; ++k) {
         dg[i][k] += u[i][k] * xh[i][k];
         db[i][k] += u[i][k];
-        u[i][k] *= g[i][k];
+        u[i][k] = at.has(i, k) ? u[i][k] * g[i][k] : 0.f;  // another lane's element adds nothing
         s1 += u[i][k];
         s2 += u[i][k] * xh[i][k];
       }

@@ -266,23 +266,22 @@ __device__ void row_top(const T* x, int n, uint32_t first, int K, Seen seen, Row
 }
 
 // One pass over x[0 .. n): the row's sums in all its threads, and what this
-// thread saw.  `v` holds batch 0 and comes back with that of `then` (null: with
-// nothing), in flight while the row is finished.
+// thread saw.
 template <typename T, int THREADS>
-__device__ __forceinline__ Soft row_pass(const T* x, int n, const T* then, Batch<T, THREADS>& v, Seen& seen,
-                                         RowShared<THREADS>& sh) {
+__device__ __forceinline__ Soft row_pass(const T* x, int n, Seen& seen, RowShared<THREADS>& sh) {
   constexpr int N = Vec<T>::N;
   const int tid = threadIdx.x % THREADS;
   const int packs = n / N, batches = (packs + THREADS * kUnroll - 1) / (THREADS * kUnroll);
   Soft a = {-INFINITY, 0.f, 0.f};
   seen = {-INFINITY, -INFINITY, -INFINITY, -1, -1};
+  Batch<T, THREADS> v;
+  if (batches) v.load(x, 0, packs);
   float tail = -INFINITY;
   if (packs * N + tid < n) tail = to_f(x[packs * N + tid]);
   for (int b = 0; b < batches; ++b) {
     float f[kUnroll * N];
     v.get(b, packs, f);
-    const bool more = b + 1 < batches;  // in flight while this batch is added
-    if (more || then) v.load(more ? x : then, more ? b + 1 : 0, packs);
+    if (b + 1 < batches) v.load(x, b + 1, packs);  // in flight while this batch is added
     float largest = f[0];
 #pragma unroll
     for (int k = 1; k < kUnroll * N; ++k) largest = fmaxf(largest, f[k]);
@@ -351,17 +350,13 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256, 5) void logprobs_ker
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
   RowShared<THREADS>& sh = shared[group];
   const int64_t step = (int64_t)gridDim.x * ROWS;
-  int64_t row = (int64_t)blockIdx.x * ROWS + group;
-  const int packs = a.V / Vec<T>::N;
-  Batch<T, THREADS> v;
-  if (row < a.N && packs) v.load(static_cast<const T*>(a.x) + row * a.ldx, 0, packs);
-  for (; row < a.N; row += step) {
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + group; row < a.N; row += step) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const int64_t t = target_of(a.target64, a.target32, row);
     const bool has = t >= 0 && t < a.V;
     const float given = has ? to_f(x[t]) : 0.f;  // the target's logit, on its way during the pass
     Seen seen;
-    const Soft r = row_pass<T, THREADS>(x, a.V, row + step < a.N ? x + step * a.ldx : nullptr, v, seen, sh);
+    const Soft r = row_pass<T, THREADS>(x, a.V, seen, sh);
     if (a.K) row_top<T, THREADS>(x, a.V, 0, a.K, seen, sh);
     row_write<T, THREADS>(a, row, r, has, given, sh);
     row_sync<THREADS>();
@@ -381,9 +376,7 @@ __global__ __launch_bounds__(256) void logprobs_part_kernel(TokenLogprobs a, int
   const int lo = part * span, n = min(span, a.V - lo);
   const T* x = static_cast<const T*>(a.x) + row * a.ldx + lo;
   Seen seen;
-  Batch<T, 256> v;
-  if (n >= Vec<T>::N) v.load(x, 0, n / Vec<T>::N);
-  const Soft r = row_pass<T, 256>(x, n, nullptr, v, seen, sh);
+  const Soft r = row_pass<T, 256>(x, n, seen, sh);
   const int K = min(a.K, n);
   if (K) row_top<T, 256>(x, n, (uint32_t)lo, K, seen, sh);
   PartSums* sums = static_cast<PartSums*>(a.work);
@@ -532,7 +525,7 @@ void fwd_typed(const TokenLogprobs& a, hipStream_t s) {
   // chip (8000: 25 us against 31 us; 30522: 81 against 64), else 256 up to
   // 64 KB (30522: 64 against 83 us with 512) and 512 above (128000: 188
   // against 194; 130 rows: 16 against 20).
-  const int64_t few = (a.N + 3) / 4;
+  const int64_t few = ((int64_t)a.N + 3) / 4;
   if (a.V <= 2048 || (a.V <= 16384 && a.N >= 2048))
     logprobs_kernel<T, 64><<<(unsigned)(few < cap ? few : cap), 256, 0, s>>>(a);
   else if ((int64_t)a.V * (int64_t)sizeof(T) <= 65536)
