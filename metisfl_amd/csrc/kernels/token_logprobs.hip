@@ -17,8 +17,8 @@
 // A list that overflows (constant rows) takes K passes over the row instead.
 //
 // Measured (a copy of 1 GiB: 5.0 TB/s):
-//   2560 x 30522   bf16  forward 33 us, 4.8 TB/s   backward 69 us, 4.5 TB/s
-//   8192 x 128000  bf16  forward 375 us with 4 alternatives, 5.6 TB/s   backward 765 us, 5.5 TB/s
+//   2560 x 30522   bf16  forward 26 us, 6.0 TB/s   backward 69 us, 4.5 TB/s
+//   8192 x 128000  bf16  forward 349 us with 4 alternatives, 6.0 TB/s   backward 795 us, 5.3 TB/s
 //   509 x 50021    fp32  forward 23 us with 20 alternatives, 4.4 TB/s
 //   1 x 30522      bf16  forward 7.6 us with 5 alternatives: 3.9 us for the pass,
 //                        0.5 for the bound, 2 for the list, 0.9 to rank and write
@@ -28,6 +28,8 @@
 // ranks lowest among the alternatives.  Sums, maxima and logs are fp32.
 #include "kernels/elem.h"
 #include "kernels/lm.h"
+
+#include <type_traits>
 
 namespace mfl {
 namespace {
@@ -439,10 +441,10 @@ int part_span(int N, int V, int type) {
 }
 
 // Backward: THREADS threads take a batch of a row; p is recomputed from the
-// row's maximum and sum.  The target's and the alternatives' own terms are
-// added by a rewrite of their elements behind a barrier, by the threads'
-// workgroup (wave) that wrote them.  The gradient is streamed out (2560 x
-// 30522 bf16 75 -> 68 us, 8192 x 128000 830 -> 755 us, 5.6 TB/s).
+// row's maximum and sum, and a thread whose pack has the target or an
+// alternative adds its own term (the alternatives of the batch are a mask of
+// the row's, so a pack asks about few).  The gradient is streamed out (2560 x
+// 30522 bf16 75 -> 69 us, 8192 x 128000 830 -> 795 us, 5.3 TB/s).
 template <typename T, int THREADS>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(TokenLogprobsBwd a, int parts) {
   constexpr int N = Vec<T>::N, SPAN = THREADS * kUnroll, GROUPS = 256 / THREADS;
@@ -457,15 +459,21 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(TokenLogprobsBwd a, i
     const int packs = a.V / N;
     Batch<T, THREADS> v;
     if (packs) v.load(x, part, packs);
-    const int64_t t = target_of(a.target64, a.target32, row);
-    const bool has = t >= 0 && t < a.V;
     const float m = a.stats[3 * row], s = a.stats[3 * row + 1];
     const bool empty = m == -INFINITY && s == 0.f;
-    const float dl = has && a.d_logp ? a.d_logp[row] : 0.f;
+    int64_t t = target_of(a.target64, a.target32, row);
+    t = t >= 0 && t < a.V && a.d_logp && !empty ? t : -1;
+    const float dl = t >= 0 ? a.d_logp[row] : 0.f;
     const float dh = a.d_entropy ? a.d_entropy[row] : 0.f;
+    const int lo = part * SPAN * N, hi = part == parts - 1 ? a.V : lo + SPAN * N;
     float all = dl;
+    uint32_t here = 0;  // the alternatives of this batch
     if (a.d_top)
-      for (int k = 0; k < a.K; ++k) all += a.d_top[row * a.K + k];
+      for (int k = 0; k < a.K; ++k) {
+        all += a.d_top[row * a.K + k];
+        const int64_t j = a.top_ids[row * a.K + k];
+        if (j >= lo && j < hi && !empty) here |= 1u << k;
+      }
     // dx_j = -p_j (all + dh (log p_j + entropy)) + own terms
     const float inv = 1.f / s, base = empty ? 0.f : m;
     const float ent = a.stats[3 * row + 2] - logf(s);
@@ -475,39 +483,47 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(TokenLogprobsBwd a, i
       if (dh != 0.f) w = fmaf(dh, fmaxf(d, -1e4f) + ent, w);
       return empty ? 0.f : -p * w;
     };
+    // together, the waves' stores run along the row (8192 x 128000 bf16: 795 us against 838 us)
+    row_sync<THREADS>();
+    // the own terms of n elements from column j
+    auto add_own = [&](int j, auto n, float* f) {
+      auto add = [&](int64_t id, float d) {
+        const int64_t e = id - j;
+        if (e >= 0 && e < n) {
+#pragma unroll
+          for (int k = 0; k < n; ++k) f[k] += k == e ? d : 0.f;
+        }
+      };
+      if (t >= 0) add(t, dl);
+      for (uint32_t left = here; left; left &= left - 1) {
+        const int k = __ffs(left) - 1;
+        add(a.top_ids[row * a.K + k], a.d_top[row * a.K + k]);
+      }
+    };
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int i = part * SPAN + u * THREADS + tid;
       if (i < packs) {
+        float f[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[k] = grad(to_f(v.v[u].e[k]));
+        add_own(i * N, std::integral_constant<int, N>(), f);
         Pack<T, N> o;
 #pragma unroll
-        for (int k = 0; k < N; ++k) o.e[k] = from_f<T>(grad(to_f(v.v[u].e[k])));
+        for (int k = 0; k < N; ++k) o.e[k] = from_f<T>(f[k]);
         stream_pack<T, N>(dx + (int64_t)i * N, o);
       }
     }
-    const int behind = packs * N;  // what is left of V, and the columns behind it: the last part's
+    // what is left of V, and the columns behind it: the last part's
     if (part == parts - 1)
-      for (int j = behind + tid; j < a.C; j += THREADS) dx[j] = from_f<T>(j < a.V ? grad(to_f(x[j])) : 0.f);
-    row_sync<THREADS>();
-    const int lo = part * SPAN * N, hi = part == parts - 1 ? a.V : lo + SPAN * N;
-    const int own = a.d_top ? a.K : 0;
-    // thread i: alternative i; the last one: the target, unless an alternative
-    // is the target (its thread adds both)
-    for (int i = tid; i <= own; i += THREADS) {
-      const int64_t j = i < own ? a.top_ids[row * a.K + i] : (has ? t : -1);
-      if (j < lo || j >= hi || empty) continue;
-      float extra = i < own ? a.d_top[row * a.K + i] : dl;
-      bool mine = true;
-      for (int k = 0; k < own; ++k)
-        if (k != i && a.top_ids[row * a.K + k] == j) {
-          if (k < i) mine = false;  // the lowest place adds for all of them
-          extra += a.d_top[row * a.K + k];
+      for (int j = packs * N + tid; j < a.C; j += THREADS) {
+        float f = 0.f;
+        if (j < a.V) {
+          f = grad(to_f(x[j]));
+          add_own(j, std::integral_constant<int, 1>(), &f);
         }
-      if (!mine) continue;
-      if (i < own && has && t == j) extra += dl;
-      dx[j] = from_f<T>(grad(to_f(x[j])) + extra);
-    }
-    row_sync<THREADS>();
+        dx[j] = from_f<T>(f);
+      }
   }
 }
 
