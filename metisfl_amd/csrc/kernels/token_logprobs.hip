@@ -540,11 +540,12 @@ void fwd_typed(const TokenLogprobs& a, hipStream_t s) {
   // a wave where rows are short, up to 16384 if there are enough to fill the
   // chip (8000: 25 us against 31 us; 30522: 81 against 64), else 256 up to
   // 64 KB (30522: 64 against 83 us with 512) and 512 above (128000: 188
-  // against 194; 130 rows: 16 against 20).
+  // against 194; 130 rows: 16 against 20) and for long rows that do not fill
+  // the chip (one row of 30522: 7.8 against 8.4).
   const int64_t few = ((int64_t)a.N + 3) / 4;
   if (a.V <= 2048 || (a.V <= 16384 && a.N >= 2048))
     logprobs_kernel<T, 64><<<(unsigned)(few < cap ? few : cap), 256, 0, s>>>(a);
-  else if ((int64_t)a.V * (int64_t)sizeof(T) <= 65536)
+  else if ((int64_t)a.V * (int64_t)sizeof(T) <= 65536 && (a.V <= 16384 || a.N > 128))
     logprobs_kernel<T, 256><<<(unsigned)(a.N < cap ? a.N : cap), 256, 0, s>>>(a);
   else
     logprobs_kernel<T, 512><<<(unsigned)(a.N < cap ? a.N : cap), 512, 0, s>>>(a);
