@@ -539,6 +539,60 @@ def test_adamw_refusals():
         MultiTensorAdamW(SPEC, p, lr_scale=torch.ones(1))
 
 
+# ---- past 32 bits --------------------------------------------------------------------------
+def test_layer_norm_past_32_bits():
+    """2.3e9 elements: the last rows' results are those of these rows alone."""
+    x = torch.empty(70_001, 32_768, dtype=torch.bfloat16, device=DEV)
+    x.normal_(generator=gen(31))
+    gamma = torch.rand(32_768, device=DEV)
+    y, mean, rstd = lm.layer_norm_fwd(x, gamma, gamma)
+    want = lm.layer_norm_fwd(x[-3:], gamma, gamma)
+    for a, b in zip((y, mean, rstd), want):
+        assert torch.equal(a[-3:], b)
+    dx = lm.layer_norm_bwd(y, x, mean, rstd, gamma)[0]
+    assert torch.equal(dx[-3:], lm.layer_norm_bwd(y[-3:], x[-3:], mean[-3:], rstd[-3:], gamma)[0])
+
+
+def test_token_logprobs_past_32_bits():
+    z = torch.empty(16_500, 131_073, dtype=torch.bfloat16, device=DEV)
+    z.normal_(generator=gen(32))
+    target = torch.arange(16_500, device=DEV)
+    r = lm.token_logprobs_fwd(z, target, 3)
+    d = lm.token_logprobs_bwd(z, target, r.stats, r.logp)
+    last = slice(16_370, 16_500)  # as many rows as are not split
+    want = lm.token_logprobs_fwd(z[last], target[last], 3)
+    for a, b in zip(r, want):
+        assert torch.equal(a[last], b)
+    assert torch.equal(d[last], lm.token_logprobs_bwd(z[last], target[last], want.stats, want.logp))
+
+
+def test_adamw_past_32_bits():
+    """A tensor whose states lie behind 2^32 others: the same as alone but for
+    the dither, which goes by the place."""
+    from metisfl_amd.ops.optim import _decode, _encode, _mix32
+    n, before = 300, (1 << 32) + 256
+    large = torch.empty(before, dtype=torch.bfloat16, device=DEV)  # without a gradient: untouched
+    p = torch.randn(n, generator=torch.Generator().manual_seed(33))
+    g = torch.randn(n, generator=torch.Generator().manual_seed(34))
+    dev = p.to(DEV)
+    opt = MultiTensorAdamW(SPEC, [large, dev], state_bits=8, seed=9)
+    opt.step([None, g.to(DEV)])
+    pad = lambda x: torch.nn.functional.pad(x, (0, -n % 128))  # noqa: E731
+    at = torch.arange(before, before + 384)
+    key = _mix32(torch.tensor([1 ^ 9]))
+    bits = _mix32((((at & 0xFFFFFFFF) ^ key) + (at >> 32) * 0x9E3779B1) & 0xFFFFFFFF)
+    m, v = pad(g) * (1 - 0.9), (pad(g) * (1 - 0.999)) * pad(g)
+    code, scale = _encode(m, bits & 0xFFFF, False)
+    same_bits(opt.m[before:], code)
+    same_bits(opt.m_scale[before // 128:], scale)
+    code, scale = _encode(v.double().sqrt().float(), bits >> 16, True)
+    same_bits(opt.v[before:], code)
+    assert (opt.m[:1000].float() == 0).all() and (_decode(code, scale)[n:] == 0).all()
+    alone = [p.clone()]
+    MultiTensorAdamW(SPEC, alone, state_bits=8, seed=9).step([g])
+    same_bits(dev, alone[0])
+
+
 # ---- together ------------------------------------------------------------------------------
 def test_model_gradients():
     check_step_gradients(DEV)
