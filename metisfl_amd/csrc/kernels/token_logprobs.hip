@@ -40,36 +40,48 @@ constexpr int kSplitRows = 128, kSplitWidth = 98304, kSplitGroups = 512;  // see
 
 // Running maximum m, sum of exp(x - m) and sum of exp(x - m) (x - m) log2 e.
 // exp(x - m) = exp2(x L - fl(m L)) with L = log2 e is one fused multiply-add
-// and one v_exp_f32; what fl(m L) is rounded by is a factor common to the sum,
-// taken out by soft_exact at the end, so the error of a term is a few times
-// 2^-24 of |x - m|, not of |x|.  Where m L would leave fp32 (rows masked with
-// the lowest value throughout) the difference is taken first.
+// and one v_exp_f32; what fl(m L) is rounded by (soft_off) is a factor common
+// to the sum: soft_grow exchanges it with the maximum and soft_exact takes it
+// out at the end, so the error of a term is a few times 2^-24 of |x - m|, not
+// of |x|.  Up to |m| = 4096 it is at most 2^-12 and soft_exact's first order
+// leaves 2^-25; beyond (logits of a large common part, rows masked with -1e9
+// throughout) the difference x - m is taken first, and nothing is left over.
 struct Soft {
   float m, s, t;
 };
-constexpr float kHuge = 1e38f;
+constexpr float kFar = 4096.f;
 __device__ __forceinline__ float scaled_max(float m) { return m == -INFINITY ? 0.f : m * kLog2e; }
-// the sums from maximum a.m to M >= a.m: each (x - m) log2 e grows by d
+__device__ __forceinline__ float soft_off(float m) {  // x L - fl(m L) - off = (x - m) L
+  return fabsf(m) > kFar ? 0.f : fmaf(m, kLog2e, -scaled_max(m));
+}
+// the sums to maximum M >= a.m: each exponent grows by d
+__device__ __forceinline__ void soft_shift(Soft& a, float M, float d) {
+  const float c = __builtin_amdgcn_exp2f(d);
+  a.t = c * (a.t + (c > 0.f ? d * a.s : 0.f));
+  a.s *= c;
+  a.m = M;
+}
+// of exact sums (s is 0 only where nothing but -inf was added)
 __device__ __forceinline__ void soft_raise(Soft& a, float M) {
-  if (a.s != 0.f) {  // (s is 0 only where nothing but -inf was added)
-    const float d = (a.m - M) * kLog2e, c = __builtin_amdgcn_exp2f(d);
-    a.t = c * (a.t + (c > 0.f ? d * a.s : 0.f));
-    a.s *= c;
-  }
+  if (a.s != 0.f) soft_shift(a, M, (a.m - M) * kLog2e);
+  a.m = M;
+}
+// of sums with their offset
+__device__ __forceinline__ void soft_grow(Soft& a, float M) {
+  if (a.s != 0.f) soft_shift(a, M, (a.m - M) * kLog2e - soft_off(a.m) + soft_off(M));
   a.m = M;
 }
 __device__ __forceinline__ void soft_exact(Soft& a) {
-  const float ml = scaled_max(a.m);
-  const float off = fabsf(a.m) > kHuge ? 0.f : fmaf(a.m, kLog2e, -ml);  // x L - fl(m L) - off = (x - m) L
-  const float c = fmaf(-off, kLn2, 1.f);                              // 2^-off
+  const float off = soft_off(a.m);
+  const float c = fmaf(-off, kLn2, 1.f);  // 2^-off
   a.t = c * fmaf(-off, a.s, a.t);
   a.s *= c;
 }
 // N more elements (fill: -inf) with the largest of them
 template <int N>
 __device__ __forceinline__ void soft_add(Soft& a, const float* x, float largest) {
-  if (largest > a.m) soft_raise(a, largest);
-  if (fabsf(a.m) > kHuge && a.m != -INFINITY) {
+  if (largest > a.m) soft_grow(a, largest);
+  if (fabsf(a.m) > kFar && a.m != -INFINITY) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const float d = (x[k] - a.m) * kLog2e, e = __builtin_amdgcn_exp2f(d);

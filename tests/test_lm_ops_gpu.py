@@ -284,6 +284,23 @@ def test_token_logprobs_masks(t, vocab):
     assert (d[5] == 0).all() and d[6].isnan().any() and d[7].isnan().any() and d[8].isfinite().all()
 
 
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [50, 1000, 40000, 140001])
+def test_token_logprobs_far_from_zero(t, vocab):
+    """Logits of a large common part, rows masked with -1e9 or -1e30 throughout,
+    maxima that grow along the row past +-4096."""
+    line = torch.linspace(0, 1, vocab, device=DEV)
+    noise = torch.randn(vocab, generator=gen(8), device=DEV)
+    rows = [1e5 + 3 * noise, torch.full_like(line, -1e9), torch.where(line < 0.5, -1e9, noise), 4090 + 12 * line,
+            -4102 + 12 * line, torch.full_like(line, 1e30), 1e5 + 6 * line, -1e9 + 640 * line, torch.full_like(line, -1e30),
+            2000 + noise, 300 + 9 * line]
+    z = torch.stack(rows).to(t)
+    target = torch.arange(len(rows), device=DEV) + vocab // 2
+    for k in (0, 4):
+        check_logprobs(z, target, k, vocab)
+    check_logprobs(z.flip(-1).contiguous(), target, 4, vocab)
+
+
 def test_token_logprobs_strides_and_shapes():
     z, target = make_logits(24, 3001, 3001, torch.bfloat16, 6)
     target = target % 3001
