@@ -409,6 +409,10 @@ class AdamPlan {
     const bool whole = firsts_.size() == 2 && firsts_[1] > 0 && firsts_[1] <= mfl::kAdamWhole;
     if (!whole) mfl::launch_adam_begin(a, s);
     C10_HIP_KERNEL_LAUNCH_CHECK();
+    for (size_t i = 0; i < grads.size(); ++i)  // autograd learns of the change, as of any in place
+      if (given(grads[i]))
+        for (const OptTensor& t : {OptTensor(params_[i]), mirrors_[i]})
+          if (given(t) && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     mfl::AdamGrads g;
     for (size_t part = 0; part + 1 < firsts_.size(); ++part) {
       const size_t lo = part * mfl::kAdamGrads, hi = std::min(grads.size(), lo + mfl::kAdamGrads);

@@ -533,6 +533,27 @@ def test_adamw_in_a_graph(bits):
     assert int(a.step_count) == 5
 
 
+def test_adamw_step_between_forward_and_backward():
+    """A backward through a parameter that a step has changed is refused, as after any change in place."""
+    w = torch.randn(8, 8, generator=gen(30), device=DEV).requires_grad_()
+    idle = torch.randn(8, 8, generator=gen(31), device=DEV).requires_grad_()
+    copy = torch.zeros(8, 8, device=DEV, dtype=torch.bfloat16)
+    opt = MultiTensorAdamW(OptimizerSpec(kind="adam"), [w, idle], mirrors=[copy, None])
+    loss, other = (w * w).sum(), (idle * idle).sum()
+    opt.step([torch.ones_like(w), None])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    other.backward()
+    assert torch.equal(idle.grad, 2 * idle.detach()) and copy._version > 0
+    with torch.inference_mode():
+        p = torch.ones(300, device=DEV)
+        MultiTensorAdamW(OptimizerSpec(kind="adam"), [p]).step([torch.ones_like(p)])
+        assert (p < 1).all()
+        y = lm.layer_norm(torch.randn(3, 40, device=DEV))
+        r = lm.token_logprobs(torch.randn(3, 40, device=DEV), torch.arange(3, device=DEV), 2)
+        assert y.isfinite().all() and all(v.isfinite().all() for v in r)
+
+
 def test_adamw_refusals():
     p = [torch.zeros(8, device=DEV)]
     opt = MultiTensorAdamW(SPEC, p)
