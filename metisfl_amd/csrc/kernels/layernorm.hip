@@ -475,14 +475,20 @@ bool with_shape(int H, F&& f) {
   if constexpr (N == 4 && !BACK) {  // (backward: 32 registers of loads ahead are too many)
     MFL_LN(64, 4, N)
   }
-  MFL_LN(256, 1, N) MFL_LN(256, 2, N)
+  if constexpr (N == 8 || BACK) {
+    MFL_LN(256, 1, N)
+  }
+  MFL_LN(256, 2, N)
   if constexpr (N == 4) {
     MFL_LN(256, 4, N)
   }
   if constexpr (N == 8 && !BACK) {
     MFL_LN(256, 3, N)
   }
-  MFL_LN(1024, 1, N) MFL_LN(1024, 2, N)
+  if constexpr (N == 8) {
+    MFL_LN(1024, 1, N)
+  }
+  MFL_LN(1024, 2, N)
   if constexpr (N == 4) {
     MFL_LN(1024, 4, N)
   }
