@@ -342,25 +342,17 @@ class AdamPlan {
     }
     firsts_.push_back((int64_t)list.size());
     TORCH_CHECK(list.size() < (size_t)1 << 24, "the parameters have too many elements for one optimizer");
+    total_ = total;
     bits_ = given(m_scale) ? 8 : 32;
-    const auto st = bits_ == 8 ? torch::kFloat8_e4m3fn : torch::kFloat32;
-    for (const Tensor* t : {&m_, &v_}) {
-      same_device(*t, first, "a state");
-      TORCH_CHECK(t->scalar_type() == st && t->is_contiguous() && t->numel() == total, "state buffer");
-    }
     if (bits_ == 8) {
       TORCH_CHECK(given(v_scale), "8-bit states need both scales");
-      vector_of(*m_scale, first, torch::kFloat32, total / mfl::kAdamBlock, "m_scale");
-      vector_of(*v_scale, first, torch::kFloat32, total / mfl::kAdamBlock, "v_scale");
       m_scale_ = *m_scale;
       v_scale_ = *v_scale;
     }
-    vector_of(step_, first, torch::kInt32, 1, "step");
-    if (given(lr_scale)) {
-      vector_of(*lr_scale, first, torch::kFloat32, 1, "lr_scale");
-      lr_scale_ = *lr_scale;
-    }
-    for (const mfl::AdamTensor& t : table) pointers_.push_back(t.p);
+    if (given(lr_scale)) lr_scale_ = *lr_scale;
+    check_states();
+    for (const Tensor& p : params_) held_.emplace_back(p);
+    for (const OptTensor& q : mirrors_) held_.push_back(given(q) ? Held(*q) : Held());
     // one copy: the table, the chunks, and zeros for the scalars and the arrivals
     const size_t tb = table.size() * sizeof(table[0]), cb = list.size() * sizeof(mfl::AdamChunk);
     Tensor host = torch::zeros({(int64_t)(tb + cb + sizeof(mfl::AdamScalars) + sizeof(int))}, torch::kUInt8);
@@ -376,14 +368,17 @@ class AdamPlan {
     const Tensor& first = params_[0];
     TORCH_CHECK(grads.size() == params_.size(), "got ", grads.size(), " gradients for ", params_.size(), " parameters");
     for (size_t i = 0; i < grads.size(); ++i) {
-      TORCH_CHECK(params_[i].data_ptr() == pointers_[i], "parameter ", i, " has another storage than at construction");
+      TORCH_CHECK(held_[i].same(params_[i]), "parameter ", i, " has another storage, size or type than at construction");
+      TORCH_CHECK(!given(mirrors_[i]) || held_[grads.size() + i].same(*mirrors_[i]), "mirror ", i,
+                  " has another storage, size or type than at construction");
       if (!given(grads[i])) continue;
       const Tensor& g = *grads[i];
       same_device(g, first, "a gradient");
       elem_type(g, "a gradient");
-      TORCH_CHECK(g.is_contiguous() && g.numel() == params_[i].numel(), "gradient ", i,
-                  " must be contiguous with its parameter's ", params_[i].numel(), " elements");
+      TORCH_CHECK(g.is_contiguous() && g.numel() == held_[i].numel, "gradient ", i,
+                  " must be contiguous with its parameter's ", held_[i].numel, " elements");
     }
+    check_states();
     c10::DeviceGuard guard(first.device());
     const hipStream_t s = stream_of(first);
     mfl::AdamStep a{};
@@ -428,10 +423,37 @@ class AdamPlan {
   }
 
  private:
+  // A tensor as the device table has it; a kernel goes by the table, so a step
+  // refuses one that is another by then (moved, cut, of another type).
+  struct Held {
+    void* p = nullptr;
+    int64_t numel = 0;
+    torch::ScalarType type = torch::kFloat32;
+    Held() = default;
+    explicit Held(const Tensor& t) : p(t.data_ptr()), numel(t.numel()), type(t.scalar_type()) {}
+    bool same(const Tensor& t) const {
+      return t.data_ptr() == p && t.numel() == numel && t.scalar_type() == type && t.is_contiguous();
+    }
+  };
+
+  void check_states() const {
+    const Tensor& first = params_[0];
+    const auto st = bits_ == 8 ? torch::kFloat8_e4m3fn : torch::kFloat32;
+    vector_of(m_, first, st, total_, "state m");
+    vector_of(v_, first, st, total_, "state v");
+    if (bits_ == 8) {
+      vector_of(m_scale_, first, torch::kFloat32, total_ / mfl::kAdamBlock, "m_scale");
+      vector_of(v_scale_, first, torch::kFloat32, total_ / mfl::kAdamBlock, "v_scale");
+    }
+    vector_of(step_, first, torch::kInt32, 1, "step");
+    if (lr_scale_.defined()) vector_of(lr_scale_, first, torch::kFloat32, 1, "lr_scale");
+  }
+
   std::vector<Tensor> params_;
   std::vector<OptTensor> mirrors_;
   Tensor m_, v_, m_scale_, v_scale_, step_, lr_scale_, tables_;
-  std::vector<void*> pointers_;  // the parameters' storage, as the table has it
+  std::vector<Held> held_;       // the parameters, then their mirrors
+  int64_t total_ = 0;            // elements of a state's buffer
   size_t chunks_at_ = 0, scalars_at_ = 0;
   std::vector<int64_t> firsts_;  // first chunk of each launch's tensors, and the end
   int bits_ = 32;

@@ -155,8 +155,9 @@ class MultiTensorAdamW:
     (csrc/kernels/multi_adamw.hip).
 
     ``params``: contiguous float32 or bfloat16 tensors on one device, updated
-    in place, no two of them sharing memory; they keep their storage for the
-    optimizer's life (a step refuses one that was moved).  ``decay``: which of
+    in place, no two of them sharing memory; they and their mirrors keep storage,
+    size and type for the optimizer's life (a step refuses one that was moved,
+    cut or cast).  ``decay``: which of
     them take ``spec.weight_decay`` (default: all).  ``mirrors``: a
     bfloat16 copy of each parameter (or None) that the step refreshes.
     ``lr_scale``: a float32 device tensor of one element that the step
@@ -215,7 +216,7 @@ class MultiTensorAdamW:
         self.step_count = zeros(1, torch.int32)
         self.lr_scale = lr_scale
         self._plan = None
-        self._pointers = [p.data_ptr() for p in self.params]
+        self._held = [_storage_of(t) for t in self.params + self.mirrors]
         if dev.type == "cuda":
             self._plan = ops().AdamPlan(self.params, self.mirrors, self.weight_decays, self.m, self.v,
                                         self.m_scale, self.v_scale, self.step_count, lr_scale, self.offsets)
@@ -258,9 +259,11 @@ class MultiTensorAdamW:
     def _reference(self, grads) -> None:
         if len(grads) != len(self.params):
             raise ValueError(f"got {len(grads)} gradients for {len(self.params)} parameters")
-        for i, (p, g) in enumerate(zip(self.params, grads)):
-            if p.data_ptr() != self._pointers[i]:
-                raise ValueError(f"parameter {i} has another storage than at construction")
+        n = len(self.params)
+        for i, (p, q, g) in enumerate(zip(self.params, self.mirrors, grads)):
+            for what, t, held in (("parameter", p, self._held[i]), ("mirror", q, self._held[n + i])):
+                if _storage_of(t) != held:
+                    raise ValueError(f"{what} {i} has another storage, size or type than at construction")
             if g is None:
                 continue
             if g.dtype not in (torch.float32, torch.bfloat16, torch.float16) or not g.is_contiguous() \
@@ -307,6 +310,11 @@ class MultiTensorAdamW:
             p.copy_(w.view(p.shape))
             if self.mirrors[i] is not None:
                 self.mirrors[i].copy_(w.view(self.mirrors[i].shape))
+
+
+def _storage_of(t: torch.Tensor | None):
+    """What a tensor's place, size and type are told by."""
+    return None if t is None else (t.data_ptr(), t.numel(), t.dtype, t.is_contiguous())
 
 
 def _mix32(x: torch.Tensor) -> torch.Tensor:

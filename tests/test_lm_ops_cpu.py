@@ -365,3 +365,42 @@ def check_user_fit(device):
 
 def test_user_fit():
     check_user_fit("cpu")
+
+
+# ---- tensors that changed under the optimizer ------------------------------------------------
+def changed_tensors(device):
+    """(optimizer, gradients) whose parameter or mirror is another than at construction."""
+    def make(change, bits):
+        p, q = torch.ones(300, device=device), torch.zeros(300, dtype=torch.bfloat16, device=device)
+        opt = MultiTensorAdamW(SPEC, [p], state_bits=bits, mirrors=[q])
+        change(p, q)
+        return opt, [torch.ones(p.numel(), device=device)]
+
+    def move_mirror(p, q):
+        q.data = torch.zeros(300, dtype=torch.bfloat16, device=device)
+
+    def cut_mirror(p, q):
+        q.data = q.data[:100]
+
+    def cut(p, q):
+        p.data = p.data[:100]
+
+    def cast(p, q):
+        p.data = p.data.view(torch.bfloat16)[:300]
+
+    def spread(p, q):
+        p.data = p.data.view(30, 10).t()
+    for change in (move_mirror, cut_mirror, cut, cast, spread):
+        for bits in (32, 8):
+            yield make(change, bits)
+
+
+def check_changed_tensors(device, error):
+    for opt, grads in changed_tensors(device):
+        with pytest.raises(error, match="another storage, size or type"):
+            opt.step(grads)
+        assert int(opt.step_count) == 0 and (opt.m.float() == 0).all()
+
+
+def test_adamw_refuses_changed_tensors():
+    check_changed_tensors("cpu", ValueError)

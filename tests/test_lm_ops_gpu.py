@@ -728,3 +728,20 @@ def test_results_on_another_stream():
         assert torch.equal(a, b)
     assert torch.equal(d, lm.token_logprobs_bwd(z, target, want.stats, want.logp))
     assert math.isfinite(float(d.float().sum()))
+
+
+# ---- tensors that changed under the optimizer ------------------------------------------------
+def test_adamw_refuses_changed_tensors():
+    from tests.test_lm_ops_cpu import check_changed_tensors
+    check_changed_tensors(DEV, RuntimeError)
+
+
+@pytest.mark.parametrize("name", ["m", "v", "m_scale", "v_scale", "step_count", "lr_scale"])
+def test_adamw_refuses_changed_states(name):
+    p = torch.ones(300, device=DEV)
+    opt = MultiTensorAdamW(SPEC, [p], state_bits=8, lr_scale=torch.ones(1, device=DEV))
+    state = getattr(opt, name)
+    state.data = state.data[:0]
+    with pytest.raises(RuntimeError, match=name.split("_count")[0]):
+        opt.step([torch.ones_like(p)])
+    assert (p == 1).all()
