@@ -305,7 +305,7 @@ Tensor token_logprobs_bwd(const Tensor& x, const Tensor& target, const Tensor& s
 // table and chunk list, and the states' buffers.
 class AdamPlan {
  public:
-  AdamPlan(std::vector<Tensor> params, std::vector<OptTensor> mirrors, std::vector<double> decay, Tensor m, Tensor v,
+  AdamPlan(std::vector<Tensor> params, std::vector<OptTensor> mirrors, std::vector<bool> decay, Tensor m, Tensor v,
            OptTensor m_scale, OptTensor v_scale, Tensor step, OptTensor lr_scale, std::vector<int64_t> offsets)
       : params_(std::move(params)), mirrors_(std::move(mirrors)), m_(m), v_(v), step_(step) {
     TORCH_CHECK(!params_.empty(), "no parameters");
@@ -334,7 +334,7 @@ class AdamPlan {
       }
       t.offset = offsets[i];
       t.numel = p.numel();
-      t.wd = (float)decay[i];
+      t.decays = decay[i];
       t.param_type = p.scalar_type() == torch::kFloat32 ? mfl::ELEM_F32 : mfl::ELEM_BF16;
       total = offsets[i] + (p.numel() + mfl::kAdamBlock - 1) / mfl::kAdamBlock * mfl::kAdamBlock;
       if (i % mfl::kAdamGrads == 0) firsts_.push_back((int64_t)list.size());
@@ -364,7 +364,8 @@ class AdamPlan {
     tables_ = host.to(first.device());
   }
 
-  void step(const std::vector<OptTensor>& grads, double lr, double beta1, double beta2, double eps, int64_t seed) {
+  void step(const std::vector<OptTensor>& grads, double lr, double beta1, double beta2, double eps, double wd,
+            int64_t seed) {
     const Tensor& first = params_[0];
     TORCH_CHECK(grads.size() == params_.size(), "got ", grads.size(), " gradients for ", params_.size(), " parameters");
     for (size_t i = 0; i < grads.size(); ++i) {
@@ -399,6 +400,7 @@ class AdamPlan {
     a.beta2 = beta2;
     a.eps = (float)eps;
     a.lr = (float)lr;
+    a.wd = (float)wd;
     a.seed = (uint32_t)seed;
     a.state_bits = bits_;
     const bool whole = firsts_.size() == 2 && firsts_[1] > 0 && firsts_[1] <= mfl::kAdamWhole;
@@ -467,7 +469,7 @@ void register_lm(pybind11::module& m) {
   m.def("token_logprobs_fwd", &token_logprobs_fwd);
   m.def("token_logprobs_bwd", &token_logprobs_bwd);
   pybind11::class_<AdamPlan>(m, "AdamPlan")
-      .def(pybind11::init<std::vector<Tensor>, std::vector<OptTensor>, std::vector<double>, Tensor, Tensor, OptTensor,
+      .def(pybind11::init<std::vector<Tensor>, std::vector<OptTensor>, std::vector<bool>, Tensor, Tensor, OptTensor,
                           OptTensor, Tensor, OptTensor, std::vector<int64_t>>())
       .def("step", &AdamPlan::step);
 }

@@ -83,7 +83,7 @@ struct AdamTensor {                // one parameter, as the device table holds i
   uint16_t* mirror;                // bf16 copy or null
   int64_t offset;                  // of its states in the flat state buffers, a multiple of kAdamBlock
   int64_t numel;
-  float wd;
+  int decays;                      // takes the step's weight decay
   int param_type;
 };
 struct AdamChunk {
@@ -107,7 +107,7 @@ struct AdamStep {
   float* m_scale;                  // 8-bit states
   float* v_scale;
   double beta1, beta2;
-  float eps, lr;
+  float eps, lr, wd;
   uint32_t seed;
   int state_bits;
 };

@@ -289,6 +289,7 @@ __device__ __forceinline__ void adam_chunk(const AdamStep& a, const AdamTensor& 
       p[k] = (m[k] * sc.c1) / (r[k] * sc.c2 + a.eps);
     }
   }
+  const float wd = t.decays ? a.wd : 0.f;
   const int64_t at = at0 + i;
   // mix32(((at + k) ^ key) + high part), its first product by parts: at is a
   // multiple of 8, so (at + k) ^ key is (at ^ key with the low bits 0) + (k ^ the key's)
@@ -297,7 +298,7 @@ __device__ __forceinline__ void adam_chunk(const AdamStep& a, const AdamTensor& 
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float pk = to_f(in.p.e[k]);
-    p[k] = pk - (p[k] + pk * t.wd) * sc.lr;
+    p[k] = pk - (p[k] + pk * wd) * sc.lr;
     if (BITS == 8 || sizeof(PT) == 2) bits[k] = mix32_rest(base + (((uint32_t)k ^ key) & 7u) * 0x9E3779B1u);
   }
   if constexpr (BITS == 8) {

@@ -158,7 +158,8 @@ class MultiTensorAdamW:
     in place, no two of them sharing memory; they and their mirrors keep storage,
     size and type for the optimizer's life (a step refuses one that was moved,
     cut or cast).  ``decay``: which of
-    them take ``spec.weight_decay`` (default: all).  ``mirrors``: a
+    them take ``spec.weight_decay`` (default: all).  A step goes by the values
+    that ``spec`` has then.  ``mirrors``: a
     bfloat16 copy of each parameter (or None) that the step refreshes.
     ``lr_scale``: a float32 device tensor of one element that the step
     multiplies the learning rate with.
@@ -178,8 +179,7 @@ class MultiTensorAdamW:
 
     def __init__(self, spec: OptimizerSpec, params, *, state_bits: int = 32, decay=None, mirrors=None,
                  lr_scale: torch.Tensor | None = None, seed: int = 0):
-        if spec.mode not in (OPT_ADAM, OPT_ADAMW):
-            raise ValueError(f"MultiTensorAdamW needs adam or adam_weight_decay, got {spec.kind}")
+        _check_adam(spec)
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
         self.spec, self.params, self.state_bits, self.seed = spec, list(params), state_bits, int(seed) & 0xFFFFFFFF
@@ -201,8 +201,7 @@ class MultiTensorAdamW:
                        for t in self.params + self.mirrors if t is not None and t.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters and mirrors must not share memory (list a tied weight once)")
-        wd = spec.weight_decay if spec.mode == OPT_ADAMW else 0.0
-        self.weight_decays = [wd if d else 0.0 for d in decay]
+        self.decay = tuple(decay)
         self.offsets, total = [], 0
         for p in self.params:
             self.offsets.append(total)
@@ -218,7 +217,7 @@ class MultiTensorAdamW:
         self._plan = None
         self._held = [_storage_of(t) for t in self.params + self.mirrors]
         if dev.type == "cuda":
-            self._plan = ops().AdamPlan(self.params, self.mirrors, self.weight_decays, self.m, self.v,
+            self._plan = ops().AdamPlan(self.params, self.mirrors, self.decay, self.m, self.v,
                                         self.m_scale, self.v_scale, self.step_count, lr_scale, self.offsets)
 
     @torch.no_grad()
@@ -228,10 +227,12 @@ class MultiTensorAdamW:
         gradient is None stays as it is, its states too."""
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         s = self.spec
+        _check_adam(s)
+        wd = s.weight_decay if s.mode == OPT_ADAMW else 0.0
         if self._plan is not None:
-            self._plan.step(grads, s.learning_rate, s.beta1, s.beta2, s.epsilon, self.seed)
+            self._plan.step(grads, s.learning_rate, s.beta1, s.beta2, s.epsilon, wd, self.seed)
         else:
-            self._reference(grads)
+            self._reference(grads, wd)
 
     # -- states ------------------------------------------------------------------------
     def state_dict(self) -> dict:
@@ -256,7 +257,7 @@ class MultiTensorAdamW:
             t.copy_(state[k])
 
     # -- the same step on the CPU ------------------------------------------------------
-    def _reference(self, grads) -> None:
+    def _reference(self, grads, wd) -> None:
         if len(grads) != len(self.params):
             raise ValueError(f"got {len(grads)} gradients for {len(self.params)} parameters")
         n = len(self.params)
@@ -297,7 +298,7 @@ class MultiTensorAdamW:
             m = m * s.beta1 + g * (1.0 - s.beta1)
             v = v * s.beta2 + (g * (1.0 - s.beta2)) * g
             r = v.double().sqrt().float()  # correctly rounded, as the kernel's (torch's fp32 one on the CPU is not)
-            w = w - ((m * c1) / (r * c2 + s.epsilon) + w * self.weight_decays[i]) * lr
+            w = w - ((m * c1) / (r * c2 + s.epsilon) + w * (wd if self.decay[i] else 0.0)) * lr
             if self.state_bits == 8:
                 self.m[a:b], self.m_scale[blocks] = _encode(m, bits & 0xFFFF, False)
                 self.v[a:b], self.v_scale[blocks] = _encode(r, bits >> 16, True)
@@ -310,6 +311,11 @@ class MultiTensorAdamW:
             p.copy_(w.view(p.shape))
             if self.mirrors[i] is not None:
                 self.mirrors[i].copy_(w.view(self.mirrors[i].shape))
+
+
+def _check_adam(spec: OptimizerSpec) -> None:
+    if spec.mode not in (OPT_ADAM, OPT_ADAMW):
+        raise ValueError(f"MultiTensorAdamW needs adam or adam_weight_decay, got {spec.kind}")
 
 
 def _storage_of(t: torch.Tensor | None):

@@ -404,3 +404,32 @@ def check_changed_tensors(device, error):
 
 def test_adamw_refuses_changed_tensors():
     check_changed_tensors("cpu", ValueError)
+
+
+def check_changed_settings(device):
+    """A step goes by the settings of its time."""
+    p, q = torch.ones(300, device=device), torch.ones(300, device=device)
+    g = torch.ones(300, device=device)
+    spec = OptimizerSpec("adam_weight_decay", 1e-2, weight_decay=0.0, epsilon=1e-6)
+    opt = MultiTensorAdamW(spec, [p, q], decay=[True, False])
+    opt.step([g, g])
+    assert torch.equal(p, q)
+    before = p.clone()
+    spec.weight_decay = 0.5
+    opt.step([g, g])
+    # equal gradients move by lr; the decay takes lr / 2 of p more, and fp32 roundings of values near 1
+    torch.testing.assert_close(q, before - 1e-2, rtol=0, atol=1e-6)
+    torch.testing.assert_close(p, before - 1e-2 - 0.5e-2 * before, rtol=0, atol=1e-6)
+    spec.kind = "adam"  # Adam has no decay
+    before = (p - q).clone()
+    opt.step([g, g])
+    torch.testing.assert_close(p - q, before, rtol=0, atol=1e-6)
+    spec.kind = "momentum_sgd"
+    with pytest.raises(ValueError, match="momentum_sgd"):
+        opt.step([g, g])
+    spec.kind = "adam"
+    assert int(opt.step_count) == 3
+
+
+def test_adamw_follows_its_settings():
+    check_changed_settings("cpu")

@@ -745,3 +745,8 @@ def test_adamw_refuses_changed_states(name):
     with pytest.raises(RuntimeError, match=name.split("_count")[0]):
         opt.step([torch.ones_like(p)])
     assert (p == 1).all()
+
+
+def test_adamw_follows_its_settings():
+    from tests.test_lm_ops_cpu import check_changed_settings
+    check_changed_settings(DEV)
