@@ -157,9 +157,8 @@ class MultiTensorAdamW:
     ``params``: contiguous float32 or bfloat16 tensors on one device, updated
     in place, no two of them sharing memory; they and their mirrors keep storage,
     size and type for the optimizer's life (a step refuses one that was moved,
-    cut or cast).  ``decay``: which of
-    them take ``spec.weight_decay`` (default: all).  A step goes by the values
-    that ``spec`` has then.  ``mirrors``: a
+    cut or cast).  ``decay``: which of them take ``spec.weight_decay`` (default:
+    all).  A step goes by the values that ``spec`` has then.  ``mirrors``: a
     bfloat16 copy of each parameter (or None) that the step refreshes.
     ``lr_scale``: a float32 device tensor of one element that the step
     multiplies the learning rate with.
@@ -171,7 +170,9 @@ class MultiTensorAdamW:
     power of two for each 128 elements.  What lies between two codes is
     rounded up with the chance of its distance, drawn from a mix of ``seed``,
     step and place: equal seeds give equal results.  bfloat16 parameters are
-    rounded the same way.  ``step_count`` is an int32 device tensor.
+    rounded the same way.  ``step_count`` is an int32 device tensor.  The
+    tensors may be written in place; putting another in an attribute's place is
+    refused.
 
     :meth:`step` can be captured into a hipGraph with the gradients of the
     captured backward; the graph keeps the spec's values (``lr_scale`` is read
@@ -182,12 +183,12 @@ class MultiTensorAdamW:
         _check_adam(spec)
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
-        self.spec, self.params, self.state_bits, self.seed = spec, list(params), state_bits, int(seed) & 0xFFFFFFFF
+        self.spec, self.params, self.state_bits, self.seed = spec, tuple(params), state_bits, int(seed) & 0xFFFFFFFF
         if not self.params:
             raise ValueError("no parameters")
         n = len(self.params)
         decay = [True] * n if decay is None else [bool(d) for d in decay]
-        self.mirrors = [None] * n if mirrors is None else list(mirrors)
+        self.mirrors = (None,) * n if mirrors is None else tuple(mirrors)
         if len(decay) != n or len(self.mirrors) != n:
             raise ValueError(f"decay and mirrors must have one entry for each of the {n} parameters")
         dev = self.params[0].device
@@ -202,16 +203,16 @@ class MultiTensorAdamW:
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters and mirrors must not share memory (list a tied weight once)")
         self.decay = tuple(decay)
-        self.offsets, total = [], 0
+        offsets, total = [], 0
         for p in self.params:
-            self.offsets.append(total)
+            offsets.append(total)
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
+        self.offsets = tuple(offsets)
         zeros = lambda k, t: torch.zeros(k, dtype=t, device=dev)  # noqa: E731
         st = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
         self.m, self.v = zeros(total, st), zeros(total, st)
-        self.m_scale = self.v_scale = None
-        if state_bits == 8:
-            self.m_scale, self.v_scale = (zeros(total // STATE_BLOCK, torch.float32) for _ in range(2))
+        self.m_scale, self.v_scale = (zeros(total // STATE_BLOCK, torch.float32) if state_bits == 8 else None
+                                      for _ in range(2))
         self.step_count = zeros(1, torch.int32)
         self.lr_scale = lr_scale
         self._plan = None
@@ -219,6 +220,15 @@ class MultiTensorAdamW:
         if dev.type == "cuda":
             self._plan = ops().AdamPlan(self.params, self.mirrors, self.decay, self.m, self.v,
                                         self.m_scale, self.v_scale, self.step_count, lr_scale, self.offsets)
+
+    # what the device tables point to: values may change in place, another object would not be seen
+    _KEPT = frozenset(("params", "mirrors", "decay", "state_bits", "offsets", "m", "v", "m_scale", "v_scale",
+                       "step_count", "lr_scale"))
+
+    def __setattr__(self, name, value):
+        if name in self._KEPT and value is not self.__dict__.get(name, value):
+            raise AttributeError(f"{name} is kept for the optimizer's life: change its values in place")
+        super().__setattr__(name, value)
 
     @torch.no_grad()
     def step(self, grads=None) -> None:

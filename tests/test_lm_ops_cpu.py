@@ -433,3 +433,23 @@ def check_changed_settings(device):
 
 def test_adamw_follows_its_settings():
     check_changed_settings("cpu")
+
+
+def check_kept_attributes(device):
+    """The device step goes by what the optimizer was made with: another object in its place is refused, not ignored."""
+    p = torch.ones(200, device=device)
+    opt = MultiTensorAdamW(SPEC, [p], state_bits=8, lr_scale=torch.ones(1, device=device))
+    for name in ("params", "mirrors", "decay", "state_bits", "offsets", "m", "v", "m_scale", "v_scale", "step_count", "lr_scale"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(opt, name, None)
+    for kept in (opt.params, opt.mirrors, opt.decay, opt.offsets):
+        with pytest.raises(TypeError):
+            kept[0] = kept[0]
+    opt.lr_scale *= 0
+    opt.step([torch.ones_like(p)])
+    assert (p == 1).all() and int(opt.step_count) == 1
+    opt.seed = 7
+
+
+def test_adamw_keeps_its_tensors():
+    check_kept_attributes("cpu")

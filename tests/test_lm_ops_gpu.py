@@ -750,3 +750,8 @@ def test_adamw_refuses_changed_states(name):
 def test_adamw_follows_its_settings():
     from tests.test_lm_ops_cpu import check_changed_settings
     check_changed_settings(DEV)
+
+
+def test_adamw_keeps_its_tensors():
+    from tests.test_lm_ops_cpu import check_kept_attributes
+    check_kept_attributes(DEV)
