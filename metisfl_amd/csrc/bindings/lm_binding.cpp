@@ -4,6 +4,7 @@
 // Arguments are checked here before any launch; work goes to the current
 // stream of the tensors' device, whichever device is current.
 #include <torch/extension.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
@@ -77,24 +78,12 @@ int param_type(const Tensor& p, const Tensor& x, int64_t H, const char* nm) {
   return t;
 }
 
-// Small results of a call come from one allocation (each costs the host a
-// microsecond, which is a fifth of a call on one token).
-class Results {
- public:
-  Results(int64_t elements, const c10::TensorOptions& o) : all_(at::empty({elements}, o)) {}
-  Tensor next(c10::IntArrayRef sizes) {
-    auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(all_.storage()), all_.key_set(), all_.dtype());
-    t->set_sizes_contiguous(sizes);
-    t->set_storage_offset(at_);
-    at_ += t->numel();
-    TORCH_INTERNAL_ASSERT(at_ <= all_.numel());
-    return Tensor(std::move(t));
-  }
-
- private:
-  Tensor all_;
-  int64_t at_ = 0;
-};
+// A result or workspace of its own, from the allocator of the current stream
+// (or of a capture).  Straight to the device's form: through the dispatcher a
+// call of five results on one row is 1.2 us longer (6.6 against 5.3 us).
+Tensor fresh(c10::IntArrayRef sizes, const Tensor& x, torch::ScalarType dt) {
+  return Tensor(at::detail::empty_cuda(sizes, dt, x.device(), c10::nullopt));
+}
 
 c10::IntArrayRef lead_of(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
 
@@ -122,8 +111,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x, const OptTens
     TORCH_CHECK(param_type(*beta, x, r.cols, "beta") == a.param_type, "gamma and beta must have the same type");
     a.beta = beta->data_ptr();
   }
-  Results small(2 * r.rows, x.options().dtype(torch::kFloat32));
-  Tensor y = at::empty(x.sizes(), x.options()), mean = small.next(lead_of(x)), rstd = small.next(lead_of(x));
+  Tensor y = fresh(x.sizes(), x, x.scalar_type()), mean = fresh(lead_of(x), x, torch::kFloat32),
+         rstd = fresh(lead_of(x), x, torch::kFloat32);
   if (r.rows == 0) return {y, mean, rstd};
   a.x = r.p;
   a.y = y.data_ptr();
@@ -151,12 +140,11 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_bwd(const Tensor& dy, const 
   vector_of(mean, x, torch::kFloat32, r.rows, "mean");
   vector_of(rstd, x, torch::kFloat32, r.rows, "rstd");
   a.param_type = given(gamma) ? param_type(*gamma, x, r.cols, "gamma") : mfl::ELEM_F32;
-  Tensor dx = at::empty(x.sizes(), x.options());
+  Tensor dx = fresh(x.sizes(), x, x.scalar_type());
   OptTensor dgamma, dbeta;
   if (given(gamma)) {
-    Results small(2 * r.cols, gamma->options());
-    dgamma = small.next({r.cols});
-    dbeta = small.next({r.cols});
+    dgamma = fresh({r.cols}, x, gamma->scalar_type());
+    dbeta = fresh({r.cols}, x, gamma->scalar_type());
   }
   if (r.rows == 0) {
     if (given(gamma)) {
@@ -177,7 +165,7 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_bwd(const Tensor& dy, const 
   a.H = (int)r.cols;
   if (given(gamma)) {
     if (const int64_t G = mfl::layer_norm_bwd_parts(a.M, a.H, a.type)) {
-      part = at::empty({G * 2 * r.cols}, x.options().dtype(torch::kFloat32));
+      part = fresh({G * 2 * r.cols}, x, torch::kFloat32);
       a.part = part.data_ptr<float>();
     }
     a.gamma = gamma->data_ptr();
@@ -222,18 +210,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_fwd(const Tens
   c10::DeviceGuard guard(x.device());
   mfl::TokenLogprobs a{};
   a.type = elem_type(x, "logits");
-  const auto f32 = x.options().dtype(torch::kFloat32);
+  const auto f32 = torch::kFloat32;
   auto shape = lead_of(x).vec();
-  Results small(r.rows * (5 + K), f32);
-  Tensor logp = small.next(shape), entropy = small.next(shape);
+  Tensor logp = fresh(shape, x, f32), entropy = fresh(shape, x, f32);
   shape.push_back(3);
-  Tensor stats = small.next(shape);
+  Tensor stats = fresh(shape, x, f32);
   shape.back() = K;
-  Tensor top = small.next(shape), ids = at::empty(shape, x.options().dtype(torch::kInt64));
+  Tensor top = fresh(shape, x, f32), ids = fresh(shape, x, torch::kInt64);
   if (r.rows == 0) return {logp, entropy, top, ids, stats};
   Tensor work;  // parts of split rows, from the allocator of the current stream (or of a capture)
   if (const size_t bytes = mfl::token_logprobs_workspace((int)r.rows, (int)V, (int)K, a.type)) {
-    work = at::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8));
+    work = fresh({(int64_t)bytes}, x, torch::kUInt8);
     a.work = work.data_ptr();
   }
   a.x = r.p;
@@ -286,7 +273,7 @@ Tensor token_logprobs_bwd(const Tensor& x, const Tensor& target, const Tensor& s
     a.d_top = static_cast<const float*>(whole(*d_top, torch::kFloat32, N * a.K, "d_top"));
     a.top_ids = static_cast<const int64_t*>(whole(*top_ids, torch::kInt64, N * a.K, "top_ids"));
   }
-  Tensor dx = at::empty(x.sizes(), x.options());
+  Tensor dx = fresh(x.sizes(), x, x.scalar_type());
   if (N == 0) return dx;
   a.x = r.p;
   a.target64 = t.t64;

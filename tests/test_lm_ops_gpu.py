@@ -755,3 +755,31 @@ def test_adamw_follows_its_settings():
 def test_adamw_keeps_its_tensors():
     from tests.test_lm_ops_cpu import check_kept_attributes
     check_kept_attributes(DEV)
+
+
+# ---- results are tensors of their own ---------------------------------------------------------
+def test_results_share_no_memory():
+    """A result that torch resizes (``out=``) or that alone is kept has nothing to do with the others."""
+    x = torch.randn(6, 40, generator=gen(40), device=DEV)
+    w, target = torch.ones(40, device=DEV), torch.arange(6, device=DEV)
+
+    def results():
+        y, mean, rstd = lm.layer_norm_fwd(x, w, w)
+        dx, dgamma, dbeta = lm.layer_norm_bwd(x, x, mean, rstd, w)
+        r = lm.token_logprobs_fwd(x, target, 3)
+        a = x.clone().requires_grad_()
+        g, b = w.clone().requires_grad_(), w.clone().requires_grad_()
+        lm.layer_norm(a, g, b).sum().backward()
+        return [y, mean, rstd, dx, dgamma, dbeta, *r, a.grad, g.grad, b.grad]
+    want = [t.clone() for t in results()]
+    got = results()
+    places = [t.untyped_storage().data_ptr() for t in got]
+    assert len(set(places)) == len(places)
+    assert all(t.untyped_storage().nbytes() == t.numel() * t.element_size() for t in got)
+    for i, t in enumerate(results()):
+        got = results()
+        if t.dtype == torch.float32:
+            got[i].detach().resize_(0)
+            torch.full((t.numel() + 3,), 7.0, device=DEV, out=got[i].detach())
+        for j, (a, b) in enumerate(zip(got, want)):
+            assert j == i or torch.equal(a, b), (i, j)
