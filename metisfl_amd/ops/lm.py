@@ -6,12 +6,12 @@ runs; these take what a user module brings (float32 / bfloat16 / float16, any
 row stride) and return new tensors.
 
 Each operator has explicit ``*_fwd`` / ``*_bwd`` calls for static training
-steps and a differentiable form for eager modules (:func:`layer_norm`,
-:func:`token_logprobs`).  Device tensors always run the HIP kernels; CPU
-tensors run the same formulas in PyTorch (float32, or float64 for float64
-inputs), which the GPU tests compare against.  Work is issued on the current
-stream of the tensors' device and can be captured into a hipGraph; results
-repeat bit for bit."""
+steps, whose results carry no graph, and a differentiable form for eager
+modules (:func:`layer_norm`, :func:`token_logprobs`).  Device tensors always
+run the HIP kernels; CPU tensors run the same formulas in PyTorch (float32, or
+float64 for float64 inputs), which the GPU tests compare against.  Work is
+issued on the current stream of the tensors' device and can be captured into a
+hipGraph; results repeat bit for bit."""
 from __future__ import annotations
 
 from typing import NamedTuple
@@ -59,6 +59,11 @@ def layer_norm_fwd(x, gamma=None, beta=None, eps: float = 1e-5):
     without ``gamma`` the norm has no weights."""
     if x.is_cuda:
         return ops().layer_norm_fwd(x, gamma, beta, eps)
+    return _layer_norm_fwd_host(x, gamma, beta, eps)
+
+
+@torch.no_grad()
+def _layer_norm_fwd_host(x, gamma, beta, eps):
     _check_norm(x, gamma, beta)
     w = _wide(_rows(x))
     mean = w.mean(1)
@@ -79,6 +84,11 @@ def layer_norm_bwd(dy, x, mean, rstd, gamma=None):
     sums in a fixed order (no atomics)."""
     if x.is_cuda:
         return ops().layer_norm_bwd(dy, x, mean, rstd, gamma)
+    return _layer_norm_bwd_host(dy, x, mean, rstd, gamma)
+
+
+@torch.no_grad()
+def _layer_norm_bwd_host(dy, x, mean, rstd, gamma):
     _check_norm(x, gamma, None)
     if dy.shape != x.shape:
         raise ValueError(f"dy has shape {tuple(dy.shape)}, expected {tuple(x.shape)}")
@@ -161,6 +171,11 @@ def token_logprobs_fwd(logits, targets, top_k: int = 0, vocab: int | None = None
     alternatives."""
     if logits.is_cuda:
         return TokenLogprobs(*ops().token_logprobs_fwd(logits, targets, top_k, vocab))
+    return _token_logprobs_fwd_host(logits, targets, top_k, vocab)
+
+
+@torch.no_grad()
+def _token_logprobs_fwd_host(logits, targets, top_k, vocab):
     vocab = _check_logits(logits, targets, vocab, top_k)
     lead = logits.shape[:-1]
     z, t = _wide(_rows(logits)[:, :vocab]), targets.reshape(-1).long()
@@ -186,6 +201,11 @@ def token_logprobs_bwd(logits, targets, stats, d_logp=None, d_entropy=None, d_to
     or None; ``d_top`` needs the forward's ``top_ids``."""
     if logits.is_cuda:
         return ops().token_logprobs_bwd(logits, targets, stats, d_logp, d_entropy, d_top, top_ids, vocab)
+    return _token_logprobs_bwd_host(logits, targets, stats, d_logp, d_entropy, d_top, top_ids, vocab)
+
+
+@torch.no_grad()
+def _token_logprobs_bwd_host(logits, targets, stats, d_logp, d_entropy, d_top, top_ids, vocab):
     vocab = _check_logits(logits, targets, vocab)
     lead = tuple(logits.shape[:-1])
     if tuple(stats.shape) != lead + (3,):

@@ -453,3 +453,21 @@ def check_kept_attributes(device):
 
 def test_adamw_keeps_its_tensors():
     check_kept_attributes("cpu")
+
+
+# ---- the explicit calls --------------------------------------------------------------------
+def check_explicit_calls(device):
+    """``*_fwd`` / ``*_bwd`` results carry no graph, on every device; the differentiable forms do."""
+    x = torch.randn(3, 8, generator=gen(9)).to(device).requires_grad_()
+    w = torch.ones(8, device=device, requires_grad=True)
+    t = torch.arange(3, device=device)
+    y, mean, rstd = lm.layer_norm_fwd(x, w, w)
+    r = lm.token_logprobs_fwd(x, t, 2)
+    out = [y, mean, rstd, *lm.layer_norm_bwd(x, x, mean, rstd, w), *r,
+           lm.token_logprobs_bwd(x, t, r.stats, x[:, 0])]
+    assert not any(v.requires_grad for v in out)
+    assert lm.layer_norm(x, w, w).requires_grad and lm.token_logprobs(x, t).logp.requires_grad
+
+
+def test_explicit_calls_carry_no_graph():
+    check_explicit_calls("cpu")

@@ -783,3 +783,8 @@ def test_results_share_no_memory():
             torch.full((t.numel() + 3,), 7.0, device=DEV, out=got[i].detach())
         for j, (a, b) in enumerate(zip(got, want)):
             assert j == i or torch.equal(a, b), (i, j)
+
+
+def test_explicit_calls_carry_no_graph():
+    from tests.test_lm_ops_cpu import check_explicit_calls
+    check_explicit_calls(DEV)
