@@ -92,6 +92,10 @@ def _layer_norm_bwd_host(dy, x, mean, rstd, gamma):
     _check_norm(x, gamma, None)
     if dy.shape != x.shape:
         raise ValueError(f"dy has shape {tuple(dy.shape)}, expected {tuple(x.shape)}")
+    rows = x.numel() // x.shape[-1]
+    for nm, s in (("mean", mean), ("rstd", rstd)):
+        if s.numel() != rows:
+            raise RuntimeError(f"{nm} must be contiguous with {rows} elements")
     d = _wide(_rows(dy))
     xh = (_wide(_rows(x)) - mean.reshape(-1, 1)) * rstd.reshape(-1, 1)
     u = d if gamma is None else d * gamma

@@ -471,3 +471,16 @@ def check_explicit_calls(device):
 
 def test_explicit_calls_carry_no_graph():
     check_explicit_calls("cpu")
+
+
+def check_statistics_of_other_rows(device):
+    """One row's statistics are not taken for all."""
+    x, w = torch.randn(3, 8, generator=gen(9)).to(device), torch.ones(8, device=device)
+    y, mean, rstd = lm.layer_norm_fwd(x, w, w)
+    for a, b, nm in ((mean[:1], rstd, "mean"), (mean, rstd[:1], "rstd"), (mean[:0], rstd, "mean")):
+        with pytest.raises(RuntimeError, match=f"{nm} must be contiguous with 3 elements"):
+            lm.layer_norm_bwd(x, x, a, b, w)
+
+
+def test_statistics_of_other_rows():
+    check_statistics_of_other_rows("cpu")

@@ -788,3 +788,8 @@ def test_results_share_no_memory():
 def test_explicit_calls_carry_no_graph():
     from tests.test_lm_ops_cpu import check_explicit_calls
     check_explicit_calls(DEV)
+
+
+def test_statistics_of_other_rows():
+    from tests.test_lm_ops_cpu import check_statistics_of_other_rows
+    check_statistics_of_other_rows(DEV)
