@@ -464,7 +464,9 @@ bool with_shape(int H, F&& f) {
   if constexpr (N == 4 && !BACK) {
     MFL_LN(16, 4, N)
   }
-  MFL_LN(64, 1, N)
+  if constexpr (N == 8 || BACK) {
+    MFL_LN(64, 1, N)
+  }
   if constexpr (N == 8) {
     MFL_LN(64, 3, 4)
   }
