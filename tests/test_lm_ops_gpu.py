@@ -793,3 +793,116 @@ def test_explicit_calls_carry_no_graph():
 def test_statistics_of_other_rows():
     from tests.test_lm_ops_cpu import check_statistics_of_other_rows
     check_statistics_of_other_rows(DEV)
+
+
+# ---- rows in parts, larger steps and other weights -----------------------------------------------
+@pytest.mark.parametrize("t", TYPES)
+def test_token_logprobs_ties_across_parts(t):
+    """Rows long enough to be split (98304 logits), with equal logits in different parts."""
+    vocab = 140_001
+    z = torch.zeros(8, vocab, device=DEV, dtype=t)
+    at = torch.arange(vocab, device=DEV)
+    z[1] = at.remainder(3).to(t)
+    z[2, 0] = z[2, -1] = z[2, vocab // 2] = 1
+    z[3, 7::4099] = 2                                    # 35 equal ones, a few to a part
+    z[3, ::9001] = 1
+    z[4, ::2] = -0.0
+    z[5, -40:] = 3                                       # all in the last part
+    z[5, 5] = 3
+    z[6] = -INF
+    z[6, 1000::30011] = 0                                # fewer finite ones than alternatives
+    z[7] = -at.div(1024, rounding_mode="floor").to(t)
+    target = torch.tensor([0, vocab - 1, vocab // 2, 7, 1, 5, 1000, vocab - 1], device=DEV)
+    for k in (0, 1, 5, 32):
+        check_logprobs(z, target, k, vocab, grads=k == 5)
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(1, 64, 140_001), (100, 768, 98_304), (129, 40, 98_305)])
+def test_split_rows_in_two_graphs(rows, width, vocab):
+    """As test_static_step_in_two_graphs, where the forward has a workspace of its own."""
+    test_static_step_in_two_graphs(rows, width, vocab)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("sizes", [[2048 * 600 + 7, 33], [1 + (i * 997) % 5000 for i in range(800)]],
+                         ids=["chunks", "tensors"])
+def test_adamw_of_several_launches_in_a_graph(bits, sizes):
+    """More chunks than one launch begins with, and more tensors than one takes;
+    some without a gradient, some bf16 with another's mirror."""
+    params, grads = make_tensors(sizes, [torch.float32, torch.bfloat16, torch.float32], [torch.float32, torch.bfloat16], 6)
+    one, two = [p.to(DEV) for p in params], [p.to(DEV) for p in params]
+    gs = [None if i % 7 == 5 else x.to(DEV) for i, x in enumerate(grads[0])]
+    copies = [[torch.zeros(n, dtype=torch.bfloat16, device=DEV) if i % 3 == 0 else None for i, n in enumerate(sizes)]
+              for _ in range(2)]
+    scale = torch.full((1,), 0.5, device=DEV)
+    a = MultiTensorAdamW(SPEC, one, state_bits=bits, mirrors=copies[0], lr_scale=scale, seed=3)
+    b = MultiTensorAdamW(SPEC, two, state_bits=bits, mirrors=copies[1], lr_scale=scale, seed=3)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a.step(gs)
+    torch.cuda.current_stream().wait_stream(s)
+    b.step(gs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(gs)
+    for k in range(4):
+        for x, y in zip(gs, grads[k % 3]):
+            if x is not None:
+                x.copy_(y)
+        scale.fill_(0.25 * (k + 1))
+        graph.replay()
+        b.step(gs)
+        torch.cuda.synchronize()
+        for p, q in zip(one + copies[0], two + copies[1]):
+            if p is not None:
+                same_bits(p, q)
+        for name, state in a.state_dict().items():
+            same_bits(state, b.state_dict()[name])
+    assert int(a.step_count) == 5
+    for i, (p, q) in enumerate(zip(one, params)):
+        if i % 7 == 5:
+            same_bits(p, q)
+
+
+def check_norm_to_subnormals(x, gamma, beta, eps, dy):
+    """check_norm's bounds, and half a step of the subnormal results: fp16 has
+    multiples of 2^-24 alone below 2^-14 (1 row of 16384: a dgamma of -5.0023e-6
+    is -5.0068e-6 in fp16), so a rounding there is off by up to 2^-25 whatever
+    the value; 2^-134 in bf16, 2^-150 in fp32."""
+    rows, h = x.shape
+    o = oracle.layer_norm(x, gamma, beta, eps, dy)
+    y, mean, rstd = lm.layer_norm_fwd(x, gamma, beta, eps)
+    dx, dgamma, dbeta = lm.layer_norm_bwd(dy, x, mean, rstd, gamma)
+    step = oracle.half_step(x.dtype)
+    tiny = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}[x.dtype]
+    mag, xh = x.double().abs().mean(-1, keepdim=True), o["xh"].abs()
+    c = 128 * U32 * (1 + mag * o["rstd"][:, None] + xh)
+    near(mean, o["mean"], 128 * U32 * mag[:, 0], "mean")
+    near(rstd, o["rstd"], 128 * U32 * o["rstd"] * (1 + mag[:, 0] * o["rstd"]), "rstd")
+    w = torch.ones(h, device=DEV).double() if gamma is None else gamma.double()
+    near(y, o["y"], c * w.abs() + (step + 4 * U32) * (o["y"].abs() + xh * w.abs()) + tiny, "y")
+    u = (dy.double() * w).abs()
+    worst = o["rstd"][:, None] * (u + u.mean(-1, keepdim=True) + (xh + 1) * (u * (xh + 1)).mean(-1, keepdim=True))
+    near(dx, o["dx"], (4 * c.amax(-1, keepdim=True) + 128 * U32) * worst + step * o["dx"].abs() + tiny, "dx")
+    if gamma is None:
+        assert dgamma is None and dbeta is None
+        return
+    assert dgamma.dtype == gamma.dtype and dbeta.dtype == gamma.dtype
+    n = (rows / 256 + 128) * U32
+    near(dgamma, o["dgamma"], n * o["dgamma_abs"] + (dy.double().abs() * c).sum(0) + step * o["dgamma"].abs() + tiny, "dgamma")
+    near(dbeta, o["dbeta"], n * o["dbeta_abs"] + step * o["dbeta"].abs() + tiny, "dbeta")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("h", [5, 24, 128, 200, 256, 512, 700, 768, 900, 1024, 1001, 2048, 4096, 4097, 6000, 8192, 12288,
+                               16383, 16384, 16391])
+def test_layer_norm_weights_of_the_inputs_type(t, h):
+    g = gen(h + 1)
+    w, b = (torch.randn(h, generator=g, device=DEV).to(t) for _ in range(2))
+    for rows in (1, 3, 300):
+        x = (torch.randn(rows, h, generator=g, device=DEV) * 1.5 + 0.25).to(t)
+        dy = torch.randn(rows, h, generator=g, device=DEV).to(t)
+        check_norm_to_subnormals(x, w, b, 1e-5, dy)
+        check_norm_to_subnormals(x, w, None, 1e-5, dy)
+        check_norm_to_subnormals(x, None, None, 1e-5, dy)
