@@ -326,6 +326,8 @@ class MultiTensorAdamW:
 def _check_adam(spec: OptimizerSpec) -> None:
     if spec.mode not in (OPT_ADAM, OPT_ADAMW):
         raise ValueError(f"MultiTensorAdamW needs adam or adam_weight_decay, got {spec.kind}")
+    if not (0 <= spec.beta1 < 1 and 0 <= spec.beta2 < 1):
+        raise ValueError(f"beta1 and beta2 must be at least 0 and below 1, got {spec.beta1} and {spec.beta2}")
 
 
 def _storage_of(t: torch.Tensor | None):

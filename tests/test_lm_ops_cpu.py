@@ -484,3 +484,18 @@ def check_statistics_of_other_rows(device):
 
 def test_statistics_of_other_rows():
     check_statistics_of_other_rows("cpu")
+
+
+@pytest.mark.parametrize("betas", [(1.0, 0.999), (0.9, 1.0), (-0.1, 0.999), (0.9, 1.5), (0.9, float("nan"))])
+def test_adamw_refuses_betas(betas):
+    """1 / (1 - beta^t) has no value, or the moments are no means."""
+    p = torch.ones(3)
+    with pytest.raises(ValueError, match="beta"):
+        MultiTensorAdamW(OptimizerSpec("adam", beta1=betas[0], beta2=betas[1]), [p])
+    spec = OptimizerSpec("adam", beta1=0.0, beta2=0.0)
+    opt = MultiTensorAdamW(spec, [p])
+    opt.step([torch.ones(3)])
+    spec.beta1, spec.beta2 = betas
+    with pytest.raises(ValueError, match="beta"):
+        opt.step([torch.ones(3)])
+    assert int(opt.step_count) == 1
