@@ -46,8 +46,8 @@ __device__ __forceinline__ uint32_t mix32_rest(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t mix32(uint32_t x) { return mix32_rest(x * 0x9E3779B1u); }  // 2^32 / golden ratio, odd
 
-// Correctly rounded root and quotient in the range where their residuals are
-// exact (normal numbers of 2^-100 to 2^100): one Newton step on v_rsq_f32 with
+// Correctly rounded root and quotient in the range where their residuals and
+// results are normal numbers (in_range): one Newton step on v_rsq_f32 with
 // the residual x - g^2 by a fused multiply-add, and Markstein's quotient
 // correction with a correctly rounded reciprocal.  The root and the reciprocal
 // were compared with 64 bits for every one of the 2^24 significands (root:
@@ -65,7 +65,16 @@ __device__ __forceinline__ float quotient_in_range(float n, float d) {
   const float q = n * r;
   return fmaf(fmaf(-d, q, n), r, q);
 }
-constexpr uint32_t kLow = (127u - 100u) << 23, kHigh = (127u + 100u) << 23;  // magnitudes of 2^-100, 2^100
+// That range.  v from 2^-100 to 2^40 and |m| from 2^-60 to 2^50, with c1, c2 (at
+// least 1) at most 2^27 and eps at most 2^20: the denominator is between 2^-50
+// and 2^48, the quotient between 2^-108 and 2^127.
+constexpr uint32_t pow2(int e) { return (uint32_t)(127 + e) << 23; }
+__device__ __forceinline__ bool in_range(uint32_t m_low, uint32_t m_high, uint32_t v_low, uint32_t v_high) {
+  return m_low >= pow2(-60) && m_high <= pow2(50) && v_low >= pow2(-100) && v_high <= pow2(40);
+}
+__device__ __forceinline__ bool in_range(float c1, float c2, float eps) {
+  return c1 <= 0x1p27f && c2 <= 0x1p27f && eps >= 0.f && eps <= 0x1p20f;
+}
 
 // b^t by squaring, in 64 bits
 __device__ double power(double b, uint32_t t) {
@@ -267,16 +276,18 @@ __device__ __forceinline__ void adam_chunk(const AdamStep& a, const AdamTensor& 
       v[k] = in.v.e[k];
     }
   }
-  uint32_t low = kHigh, high = 0;
+  uint32_t m_low = kInf, m_high = 0, v_low = kInf, v_high = 0;  // (v has no sign but a NaN's)
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float gk = to_f(in.g.e[k]);
     m[k] = m[k] * b1 + gk * n1;
     v[k] = v[k] * b2 + (gk * n2) * gk;
-    low = min(low, min(magnitude(v[k]), magnitude(m[k])));
-    high = max(high, max(magnitude(v[k]), magnitude(m[k])));
+    m_low = min(m_low, magnitude(m[k]));
+    m_high = max(m_high, magnitude(m[k]));
+    v_low = min(v_low, __float_as_uint(v[k]));
+    v_high = max(v_high, __float_as_uint(v[k]));
   }
-  if (low >= kLow && high <= kHigh && magnitude(a.eps) <= kHigh) {
+  if (in_range(m_low, m_high, v_low, v_high) && in_range(sc.c1, sc.c2, a.eps)) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       r[k] = root_in_range(v[k]);

@@ -906,3 +906,35 @@ def test_layer_norm_weights_of_the_inputs_type(t, h):
         check_norm_to_subnormals(x, w, b, 1e-5, dy)
         check_norm_to_subnormals(x, w, None, 1e-5, dy)
         check_norm_to_subnormals(x, None, None, 1e-5, dy)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (1 - 1e-12, 0.5), (0.5, 1 - 1e-12)])
+def test_adamw_equals_the_reference_at_overflow(bits, betas):
+    """States whose quotient, or whose correction 1 / (1 - beta^t), has no fp32 value."""
+    n = 128 * 8
+    g = torch.Generator().manual_seed(22)
+    size = 2.0 ** torch.randint(20, 31, (n,), generator=g).float()
+    m = torch.where(torch.rand(n, generator=g) < 0.5, -1.0, 1.0) * size * 2.0 ** 64
+    v = 2.0 ** torch.randint(-98, -90, (n,), generator=g).float()
+    spec = OptimizerSpec("adam", 1e-2, beta1=betas[0], beta2=betas[1], epsilon=0.0)
+    params = [torch.randn(n, generator=g)]
+    dev = [p.to(DEV) for p in params]
+    a = MultiTensorAdamW(spec, params, state_bits=bits)
+    b = MultiTensorAdamW(spec, dev, state_bits=bits)
+    if bits == 32:
+        a.m.copy_(m)
+        a.v.copy_(v)
+    else:
+        a.m.copy_((m / 2.0 ** 86).to(torch.float8_e4m3fn))
+        a.m_scale.fill_(2.0 ** 86)
+        a.v.copy_((v.sqrt() * 2.0 ** 49).to(torch.float8_e4m3fn))
+        a.v_scale.fill_(2.0 ** -49)
+    b.load_state_dict(a.state_dict())
+    grad = torch.zeros(n)
+    a.step([grad])
+    b.step([grad.to(DEV)])
+    assert torch.equal(params[0].isnan(), dev[0].cpu().isnan())
+    same_bits(params[0].nan_to_num(7.0, INF, -INF), dev[0].nan_to_num(7.0, INF, -INF))
+    for name, s in a.state_dict().items():
+        same_bits(s, b.state_dict()[name])
