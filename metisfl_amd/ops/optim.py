@@ -215,6 +215,9 @@ class MultiTensorAdamW:
                                       for _ in range(2))
         self.step_count = zeros(1, torch.int32)
         self.lr_scale = lr_scale
+        if dev.type != "cuda" and lr_scale is not None and (
+                lr_scale.dtype != torch.float32 or lr_scale.numel() != 1 or lr_scale.device != dev):
+            raise ValueError("lr_scale must be a float32 tensor of one element on the parameters' device")
         self._plan = None
         self._held = [_storage_of(t) for t in self.params + self.mirrors]
         if dev.type == "cuda":
@@ -287,7 +290,7 @@ class MultiTensorAdamW:
         c2 = torch.tensor(1.0 / (1.0 - s.beta2 ** t) ** 0.5, dtype=f)
         lr = torch.tensor(s.learning_rate, dtype=f)
         if self.lr_scale is not None:
-            lr = lr * self.lr_scale[0]
+            lr = lr * self.lr_scale.reshape(())
         key = _mix32(torch.tensor([(t ^ self.seed) & 0xFFFFFFFF]))
         for i, (p, g) in enumerate(zip(self.params, grads)):
             if g is None or p.numel() == 0:

@@ -499,3 +499,20 @@ def test_adamw_refuses_betas(betas):
     with pytest.raises(ValueError, match="beta"):
         opt.step([torch.ones(3)])
     assert int(opt.step_count) == 1
+
+
+def check_scale_of_the_rate(device, error):
+    """One float32 element of any shape, beside the parameters."""
+    p, q = torch.ones(3, device=device), torch.ones(3, device=device)
+    a = MultiTensorAdamW(SPEC, [p], lr_scale=torch.tensor(0.5, device=device))
+    b = MultiTensorAdamW(SPEC, [q], lr_scale=torch.full((1,), 0.5, device=device))
+    a.step([torch.ones(3, device=device)])
+    b.step([torch.ones(3, device=device)])
+    assert torch.equal(p, q) and (p < 1).all()
+    for bad in (torch.ones(2, device=device), torch.ones(0, device=device), torch.ones(1, device=device).double()):
+        with pytest.raises(error, match="lr_scale"):
+            MultiTensorAdamW(SPEC, [p], lr_scale=bad)
+
+
+def test_adamw_scale_of_the_rate():
+    check_scale_of_the_rate("cpu", ValueError)

@@ -938,3 +938,8 @@ def test_adamw_equals_the_reference_at_overflow(bits, betas):
     same_bits(params[0].nan_to_num(7.0, INF, -INF), dev[0].nan_to_num(7.0, INF, -INF))
     for name, s in a.state_dict().items():
         same_bits(s, b.state_dict()[name])
+
+
+def test_adamw_scale_of_the_rate():
+    from tests.test_lm_ops_cpu import check_scale_of_the_rate
+    check_scale_of_the_rate(DEV, RuntimeError)
