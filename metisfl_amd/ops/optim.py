@@ -180,7 +180,7 @@ class MultiTensorAdamW:
 
     def __init__(self, spec: OptimizerSpec, params, *, state_bits: int = 32, decay=None, mirrors=None,
                  lr_scale: torch.Tensor | None = None, seed: int = 0):
-        _check_adam(spec)
+        _adam_decay(spec)
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
         self.spec, self.params, self.state_bits, self.seed = spec, tuple(params), state_bits, int(seed) & 0xFFFFFFFF
@@ -240,8 +240,7 @@ class MultiTensorAdamW:
         gradient is None stays as it is, its states too."""
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         s = self.spec
-        _check_adam(s)
-        wd = s.weight_decay if s.mode == OPT_ADAMW else 0.0
+        wd = _adam_decay(s)
         if self._plan is not None:
             self._plan.step(grads, s.learning_rate, s.beta1, s.beta2, s.epsilon, wd, self.seed)
         else:
@@ -326,11 +325,14 @@ class MultiTensorAdamW:
                 self.mirrors[i].copy_(w.view(self.mirrors[i].shape))
 
 
-def _check_adam(spec: OptimizerSpec) -> None:
-    if spec.mode not in (OPT_ADAM, OPT_ADAMW):
+def _adam_decay(spec: OptimizerSpec) -> float:
+    """The decoupled weight decay of a spec that MultiTensorAdamW takes."""
+    mode = spec.mode
+    if mode not in (OPT_ADAM, OPT_ADAMW):
         raise ValueError(f"MultiTensorAdamW needs adam or adam_weight_decay, got {spec.kind}")
     if not (0 <= spec.beta1 < 1 and 0 <= spec.beta2 < 1):
         raise ValueError(f"beta1 and beta2 must be at least 0 and below 1, got {spec.beta1} and {spec.beta2}")
+    return spec.weight_decay if mode == OPT_ADAMW else 0.0
 
 
 def _storage_of(t: torch.Tensor | None):
