@@ -50,8 +50,8 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& v) {
   __builtin_memcpy(p, &v, sizeof(v));
 }
 
-// The same past the caches' write-back (16 bytes): for results that nothing
-// reads soon, a stream of stores then does not fetch or evict lines.
+// The same past the caches' write-back (16 bytes), for results larger than the
+// caches: a stream of stores then does not fetch or evict lines.
 template <typename T, int N>
 __device__ __forceinline__ void stream_pack(T* p, const Pack<T, N>& v) {
   typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));

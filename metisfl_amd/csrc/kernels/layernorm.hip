@@ -15,11 +15,17 @@
 // workgroups' rows in a fixed order, so results repeat bit for bit (no
 // atomics).  All sums are fp32.
 //
-// Measured (a copy of 1 GiB: 5.0 TB/s, of 64 MiB, cached: 7.8 TB/s):
-//   16384 x 768   bf16  forward  10.3 us, 4.9 TB/s  backward  16.2 us, 4.7 TB/s
-//   16384 x 4096  bf16  forward  47 us,   5.6 TB/s  backward  80 us,   5.0 TB/s
-//   24576 x 5120  fp32  forward  198 us,  5.1 TB/s  backward  279 us,  5.4 TB/s
-//   1 x 768       fp32  forward  1.7 us on the GPU, 5.2 us a call
+// Measured, calls among others over three sets of inputs in turn, fp32 weights
+// (copies of 1 GiB: 4.7 to 5.1 TB/s; of 64 MiB: 5.1 TB/s over three pairs of
+// buffers in turn, 6.9 TB/s over one pair, which stays cached):
+//   16384 x 768    bf16  forward  10.7 us, 4.7 TB/s  backward  16.8 us, 4.5 TB/s
+//   16384 x 4096   bf16  forward  57 us,   4.7 TB/s  backward  83 us,   4.8 TB/s
+//   24576 x 5120   fp32  forward  199 us,  5.1 TB/s  backward  279 us,  5.4 TB/s
+//   4099 x 1001    fp16  forward  6.1 us,  2.7 TB/s  backward  12.3 us, 2.0 TB/s
+//   4096 x 16384   fp32  forward  97 us,   5.6 TB/s  backward  191 us,  4.2 TB/s
+//   2048 x 40000   bf16  forward  105 us,  3.1 TB/s  backward  240 us,  2.1 TB/s
+//   1 x 768        fp32  forward  1.8 us on the GPU, 5.2 us a call
+// Weights of the input's type: 16384 x 768 bf16 11.8 and 17.0 us.
 #include "kernels/elem.h"
 #include "kernels/lm.h"
 
@@ -436,9 +442,14 @@ __global__ __launch_bounds__(1024) void ln_wgrad_kernel(const float* __restrict_
 
 // Lanes and packs of a row, elements of a pack (16 bytes, or 8 where that
 // leaves fewer lanes idle), exactness: the fewest lanes that hold the row in
-// 16 elements each (with the weights and their sums a backward thread then
-// stays within 128 registers).  Rows of fewer elements than a pack take one
-// element a lane.
+// about 16 elements each.  A backward thread of 1024 has 128 registers, and with
+// the weights and their sums some shapes need more: fp32 above 8192 columns
+// spills 41 to 46 (4096 x 12288: 186 us, 3.2 TB/s; 4096 x 8192, which does not
+// spill: 82 us, 4.9 TB/s), 16-bit rows of 8193 to 16383 columns 6 to 12 (8192 x
+// 16000 bf16: 190 us, 4.1 TB/s; 16384 columns 164 us, 4.9), and with 16-bit
+// weights 16384 columns 2 and 769 to 1023 columns 4 to 9 (16384 x 900 bf16:
+// 26.5 us against 23.2 with fp32 weights).  Rows of fewer elements than a pack
+// take one element a lane.
 template <typename T, bool BACK, typename F>
 bool with_shape(int H, F&& f) {
   constexpr int N = Vec<T>::N;
@@ -514,8 +525,9 @@ void fwd_typed(const LayerNormFwd& a, hipStream_t s) {
 
 // Workgroups of the backward: what the chip holds at a time, fewer for few
 // rows, and one where its groups have at most four rows each, which spares the
-// second launch (one row of 768 fp32: 5.7 us a call against 8.5 us; 64 rows,
-// four to a group: 7.9 against 8.9).  Rows wider than registers hold: the parts
+// second launch (a call on one row of 768 fp32: 4.5 us against 7.4; 4 rows of
+// 1024: 4.7 against 7.5; 4 rows of 8192: 6.9 against 7.4; 64 rows of 768, four to
+// a group: 7.9 against 7.2 to 8.5).  Rows wider than registers hold: the parts
 // that the columns' sums are split into.
 template <typename T>
 int bwd_blocks(int M, int H) {

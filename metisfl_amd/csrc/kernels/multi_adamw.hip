@@ -11,8 +11,8 @@
 // tensors and holds in a captured graph.  The first launch (one thread)
 // advances the step counter and evaluates c1, c2 (in 64 bits) and the
 // rounding key once instead of in every workgroup.  Up to 512 workgroups do
-// that themselves in a single launch (six tensors of 118282 elements: 5.8 us a
-// step instead of 8.5 us in two launches; the arrivals of 50000 workgroups
+// that themselves in a single launch (six tensors of 118282 elements: 5.9 us a
+// step instead of 9.3 us in two launches; the arrivals of 50000 workgroups
 // would take longer than the step).
 //
 // 8-bit states: 128 elements share a power of two 2^E that puts their largest
@@ -26,7 +26,7 @@
 // states are kept as NaN.
 //
 // Measured: 110 million elements in 199 tensors, bf16 gradients and mirrors,
-// 592 us (5.2 TB/s) with 32-bit and 353 us (5.0 TB/s) with 8-bit states.
+// 593 us (5.2 TB/s) with 32-bit and 354 us (5.0 TB/s) with 8-bit states.
 //
 // The arithmetic is a fixed order of single fp32 operations (no contraction),
 // so results do not depend on the launch and repeat bit for bit.

@@ -14,14 +14,19 @@
 // lower bound of the K-th largest logit, and only threads whose own maximum
 // reaches it read their few elements again (from L2) and list those at or
 // above it; the list (about K long for logits without many ties) is ranked.
-// A list that overflows (constant rows) takes K passes over the row instead.
+// A list that overflows (constant rows) takes K passes over the row instead: 64
+// x 128000 bf16 zeros take 81 us with 4 alternatives and 397 us with 32, 2048 x
+// 30522 2.7 ms with 32.
 //
-// Measured (a copy of 1 GiB: 5.0 TB/s):
-//   2560 x 30522   bf16  forward 26 us, 6.0 TB/s   backward 69 us, 4.5 TB/s
-//   8192 x 128000  bf16  forward 349 us with 4 alternatives, 6.0 TB/s   backward 795 us, 5.3 TB/s
-//   509 x 50021    fp32  forward 23 us with 20 alternatives, 4.4 TB/s
-//   1 x 30522      bf16  forward 7.6 us with 5 alternatives: 3.9 us for the pass,
-//                        0.5 for the bound, 2 for the list, 0.9 to rank and write
+// Measured, calls among others over three sets of inputs in turn (copies of 1
+// GiB: 4.7 to 5.1 TB/s; a pass that only reads goes above):
+//   2560 x 30522   bf16  forward 36.7 us, 4.3 TB/s   backward 65 us, 4.8 TB/s
+//   2560 x 30522   fp32  forward 53.9 us, 5.8 TB/s   backward 117 us, 5.3 TB/s
+//   8192 x 128000  bf16  forward 348 us with 4 alternatives, 6.0 TB/s
+//                        backward 790 us, with the entropy's gradient 782, 5.3 TB/s
+//   509 x 50021    fp32  forward 24.5 us with 20 alternatives, 4.2 TB/s
+//   130 x 128000   bf16  forward 14.9 us with 5 alternatives, 2.2 TB/s
+//   1 x 30522      bf16  forward 7.0 us on the GPU with 5 alternatives, 7.4 us a call
 //
 // A row of nothing but -inf has no distribution: logp and top_logp -inf,
 // entropy 0, gradient 0.  NaN or +inf in a row makes its results NaN; NaN
@@ -440,8 +445,10 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(TokenLogprobs a, int 
 }
 // Elements of a part, or 0 for rows that are not split: only long rows that
 // leave most of the chip idle are, into batches of 256 threads, at most 64
-// (bf16, 32 rows: 200000 logits 9.9 us against 17.5 us, 65000 10 against 8.5,
-// the join's launch being 2 us).
+// (128000 bf16 logits: one row 10.4 us against 13.5 us, 32 rows 11.6 against
+// 14.4, 96 rows 15.5 against 14.8, 128 rows 16.3 against 15.0, 160 rows 18.0
+// against 15.3; 128 rows of 200000 fp32 25.8 against 25.7; 32 rows of 65000 bf16
+// 10 against 8.5, the join's launch being 2 us).
 int part_span(int N, int V, int type) {
   const int batch = 256 * kUnroll * (type == ELEM_F32 ? 4 : 8);
   if (N > kSplitRows || V < kSplitWidth) return 0;
@@ -456,7 +463,8 @@ int part_span(int N, int V, int type) {
 // row's maximum and sum, and a thread whose pack has the target or an
 // alternative adds its own term (the alternatives of the batch are a mask of
 // the row's, so a pack asks about few).  The gradient is streamed out (2560 x
-// 30522 bf16 75 -> 69 us, 8192 x 128000 830 -> 795 us, 5.3 TB/s).
+// 30522 bf16 75 -> 69 us, 8192 x 128000 830 -> 795 us): this launch alone was
+// timed, not the products that read the gradient next.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(TokenLogprobsBwd a, int parts) {
   constexpr int N = Vec<T>::N, SPAN = THREADS * kUnroll, GROUPS = 256 / THREADS;
@@ -548,12 +556,18 @@ void fwd_typed(const TokenLogprobs& a, hipStream_t s) {
     logprobs_join_kernel<T><<<a.N, 64, 0, s>>>(a, parts);
     return;
   }
-  // Threads to a row, both sides measured (bf16, 4160 rows, 5 alternatives):
-  // a wave where rows are short, up to 16384 if there are enough to fill the
-  // chip (8000: 25 us against 31 us; 30522: 81 against 64), else 256 up to
-  // 64 KB (30522: 64 against 83 us with 512) and 512 above (128000: 188
-  // against 194; 130 rows: 16 against 20) and for long rows that do not fill
-  // the chip (one row of 30522: 7.8 against 8.4).
+  // Threads to a row, both sides measured with 5 alternatives (4160 rows where
+  // none are named).  A wave where rows are short, up to 16384 if there are
+  // enough to fill the chip (fp16 2500: 14.4 us against 25.1 with 256, 8000:
+  // 21.5 against 25.5, 16000: 37.8 against 37.7, 30522: 62 against 56; fp32
+  // 2500: 13.9 against 18.2, 8000: 32.4 against 31.2, 16000: 58 against 52;
+  // 1024 x 2500 fp32: 7.2 against 7.9 the other way).  Else 256 up to 64 KB
+  // (fp16 30522: 56 against 75 with 512; fp32 16000: 130 rows 7.4 against 7.1)
+  // and 512 above (2048 x 30522 fp32: 47.8 against 50.8, 18000: 59.0 against
+  // 56.5, fp16 40000: 88 against 66 the other way) and for long rows that do not
+  // fill the chip (one row of 30522 bf16: 7.8 against 8.4; 100 x 18000 fp32: 7.4
+  // against 7.9).  The limits were set on bf16: fp32 from 8000 and rows of 64
+  // to 80 KB would be faster with 256.
   const int64_t few = ((int64_t)a.N + 3) / 4;
   if (a.V <= 2048 || (a.V <= 16384 && a.N >= 2048))
     logprobs_kernel<T, 64><<<(unsigned)(few < cap ? few : cap), 256, 0, s>>>(a);

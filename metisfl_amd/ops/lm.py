@@ -172,7 +172,8 @@ def token_logprobs_fwd(logits, targets, top_k: int = 0, vocab: int | None = None
     A target outside [0, vocab) marks a row without one: its logp is 0.  A
     row of nothing but -inf gives logp and top_logp -inf and entropy 0; NaN
     or +inf in a row makes its results NaN, and NaN ranks lowest among the
-    alternatives."""
+    alternatives.  Rows in which more than 1024 logits (256 in short rows) tie for the
+    alternatives (a head initialised to zero) are read ``top_k`` times more."""
     if logits.is_cuda:
         return TokenLogprobs(*ops().token_logprobs_fwd(logits, targets, top_k, vocab))
     return _token_logprobs_fwd_host(logits, targets, top_k, vocab)
