@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
@@ -349,6 +350,7 @@ class AdamPlan {
     chunks_at_ = tb;
     scalars_at_ = tb + cb;
     tables_ = host.to(first.device());
+    hold_on_stream();  // their own
   }
 
   void step(const std::vector<OptTensor>& grads, double lr, double beta1, double beta2, double eps, double wd,
@@ -369,6 +371,7 @@ class AdamPlan {
     check_states();
     c10::DeviceGuard guard(first.device());
     const hipStream_t s = stream_of(first);
+    hold_on_stream();
     mfl::AdamStep a{};
     uint8_t* tables = tables_.data_ptr<uint8_t>();
     a.tensors = reinterpret_cast<const mfl::AdamTensor*>(tables);
@@ -438,11 +441,24 @@ class AdamPlan {
     if (lr_scale_.defined()) vector_of(lr_scale_, first, torch::kFloat32, 1, "lr_scale");
   }
 
+  // The allocator reuses what is freed in the order of the stream that
+  // allocated it; a step on another stream may still run when the optimizer is
+  // dropped.  Nobody else can tell it of the tables.
+  void hold_on_stream() {
+    const c10::Stream now = c10::impl::VirtualGuardImpl(step_.device().type()).getStream(step_.device());
+    for (const c10::Stream& known : streams_)
+      if (known == now) return;
+    for (const Tensor& t : {tables_, m_, v_, m_scale_, v_scale_, step_})
+      if (t.defined() && !streams_.empty()) t.record_stream(now);
+    streams_.push_back(now);
+  }
+
   std::vector<Tensor> params_;
   std::vector<OptTensor> mirrors_;
   Tensor m_, v_, m_scale_, v_scale_, step_, lr_scale_, tables_;
   std::vector<Held> held_;       // the parameters, then their mirrors
   int64_t total_ = 0;            // elements of a state's buffer
+  std::vector<c10::Stream> streams_;  // that steps ran on, the first the construction's
   size_t chunks_at_ = 0, scalars_at_ = 0;
   std::vector<int64_t> firsts_;  // first chunk of each launch's tensors, and the end
   int bits_ = 32;

@@ -176,7 +176,8 @@ class MultiTensorAdamW:
 
     :meth:`step` can be captured into a hipGraph with the gradients of the
     captured backward; the graph keeps the spec's values (``lr_scale`` is read
-    by every replay)."""
+    by every replay) and points into the optimizer's states and tables: keep the
+    optimizer as long as the graph is replayed."""
 
     def __init__(self, spec: OptimizerSpec, params, *, state_bits: int = 32, decay=None, mirrors=None,
                  lr_scale: torch.Tensor | None = None, seed: int = 0):

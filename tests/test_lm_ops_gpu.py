@@ -943,3 +943,28 @@ def test_adamw_equals_the_reference_at_overflow(bits, betas):
 def test_adamw_scale_of_the_rate():
     from tests.test_lm_ops_cpu import check_scale_of_the_rate
     check_scale_of_the_rate(DEV, RuntimeError)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_dropped_while_its_step_waits(bits):
+    """A step on another stream than the construction's, the optimizer dropped
+    before it runs, its memory asked for again: the step has its tables and states."""
+    n = 128 * 5000
+    want, p = torch.ones(n, device=DEV), torch.ones(n, device=DEV)
+    g = torch.randn(n, generator=gen(50), device=DEV)
+    MultiTensorAdamW(SPEC, [want], state_bits=bits).step([g])
+    opt = MultiTensorAdamW(SPEC, [p], state_bits=bits)
+    places = {t.data_ptr() for t in opt.state_dict().values()}
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(50_000_000)  # 25 ms or more
+        opt.step([g])
+    sizes = [t.numel() * t.element_size() for t in opt.state_dict().values()]
+    del opt
+    again = [torch.empty(k, dtype=torch.uint8, device=DEV) for k in sizes + [64, 512, 4096, 8192, 16384] for _ in range(4)]
+    assert not places & {t.data_ptr() for t in again}  # (before anything is written there)
+    for t in again:
+        t.fill_(127)
+    torch.cuda.synchronize()
+    assert torch.equal(p, want) and all((t == 127).all() for t in again)
